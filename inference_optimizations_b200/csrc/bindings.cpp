@@ -236,6 +236,219 @@ void gqa_decode(const at::Tensor& q, const at::Tensor& pool, const at::Tensor& p
   CHECK_CUDA_OK(iob::gqa_decode(a, stream()));
 }
 
+// Numbers go into messages as text: streaming an integer through TORCH_CHECK crashes where torch and this extension
+// carry different C++ runtimes.
+std::string num(int64_t v) { return std::to_string(v); }
+
+// Block-sparse attention: checks shared by its entry points.
+void block_pool(const at::Tensor& pool, int64_t fmt, int64_t Hk, int64_t D) {
+  req(pool, at::kByte, "pool");
+  TORCH_CHECK(D == 128 || D == 256 || D == 512, "head_dim 128, 256 or 512, got ", num(D));
+  TORCH_CHECK(fmt >= iob::kKvBf16 && fmt <= iob::kKvNvfp4, "GQA pool format, got ", num(fmt));
+  TORCH_CHECK(pool.dim() == 4 && pool.is_contiguous() && pool.size(1) == Hk && pool.size(2) == 2 &&
+                  2 * pool.size(3) == iob::gqa_block_bytes(static_cast<int>(fmt), static_cast<int>(D), 64),
+              "pool uint8 [pages, Hk, 2, part bytes], contiguous");
+  TORCH_CHECK(pool.size(0) < (1 << 25), "pool pages");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(pool.data_ptr()) % 16 == 0, "pool must be 16-byte aligned");
+}
+
+void block_bounds(const at::Tensor& codes, const at::Tensor& scale, int64_t pages, int64_t Hk, int64_t D) {
+  req(codes, at::kChar, "codes");
+  req(scale, at::kBFloat16, "scale");
+  TORCH_CHECK(codes.dim() == 4 && codes.is_contiguous() && codes.size(0) == pages && codes.size(1) == Hk &&
+                  codes.size(2) == 2 && codes.size(3) == D, "codes int8 [pages, Hk, 2, D], contiguous");
+  TORCH_CHECK(scale.dim() == 2 && scale.is_contiguous() && scale.size(0) == pages && scale.size(1) == Hk,
+              "scale bf16 [pages, Hk], contiguous");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0, "codes must be 16-byte aligned");
+}
+
+// Per-group inputs: q [B * n_q, Hq, D] (rows may be strided), page table, kv_len [B], req_idx [B].
+void block_groups(const at::Tensor& q, const at::Tensor& page_table, const c10::optional<at::Tensor>& req_idx,
+                  const at::Tensor& kv_len, int64_t n_q, int64_t Hk) {
+  req(q, at::kBFloat16, "q");
+  req(page_table, at::kInt, "page_table");
+  req(kv_len, at::kInt, "kv_len");
+  TORCH_CHECK(q.dim() == 3 && q.stride(2) == 1 && q.stride(1) == q.size(2) && q.stride(0) >= 0,
+              "q [B * n_q, Hq, D] with contiguous heads");
+  TORCH_CHECK(q.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+              "q rows must be 16-byte aligned");
+  TORCH_CHECK(kv_len.dim() == 1 && kv_len.is_contiguous() && n_q >= 1 && q.size(0) == kv_len.size(0) * n_q,
+              "kv_len [B], q rows B * n_q");
+  TORCH_CHECK(Hk >= 1 && q.size(1) % Hk == 0 && n_q * (q.size(1) / Hk) <= 16,
+              "n_q * (Hq / Hk) must be whole and at most 16");
+  TORCH_CHECK(page_table.dim() == 2 && page_table.is_contiguous() && page_table.size(0) >= 1 &&
+                  page_table.size(1) >= 1 && page_table.size(1) < (1 << 25), "page_table [rows, pages], contiguous");
+  if (req_idx.has_value()) {
+    req(*req_idx, at::kInt, "req_idx");
+    TORCH_CHECK(req_idx->dim() == 1 && req_idx->is_contiguous() && req_idx->size(0) == kv_len.size(0), "req_idx [B]");
+  } else {
+    TORCH_CHECK(page_table.size(0) >= kv_len.size(0), "page_table needs a row per group without req_idx");
+  }
+}
+
+void block_append(const at::Tensor& qkv, c10::optional<at::Tensor> q_norm, c10::optional<at::Tensor> k_norm,
+                  const at::Tensor& cos_sin, const at::Tensor& pos, const at::Tensor& slot, at::Tensor q_out,
+                  at::Tensor pool, at::Tensor codes, at::Tensor scale, int64_t fmt, double k_scale, double v_scale,
+                  int64_t Hq, int64_t Hk, int64_t D, double eps, bool plus_one) {
+  req(qkv, at::kBFloat16, "qkv");
+  req(cos_sin, at::kFloat, "cos_sin");
+  req(pos, at::kInt, "pos");
+  req(slot, at::kInt, "slot");
+  req(q_out, at::kBFloat16, "q_out");
+  block_pool(pool, fmt, Hk, D);
+  block_bounds(codes, scale, pool.size(0), Hk, D);
+  TORCH_CHECK(Hq >= 1 && Hk >= 1, "head counts");
+  TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) >= (Hq + 2 * Hk) * D, "qkv [T, (Hq + 2 Hk) D]");
+  TORCH_CHECK(qkv.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
+              "qkv rows must be 16-byte aligned");
+  TORCH_CHECK(cos_sin.dim() == 2 && cos_sin.is_contiguous() && cos_sin.size(1) == D &&
+                  reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) % 16 == 0, "cos_sin [positions, D], contiguous");
+  TORCH_CHECK(pos.is_contiguous() && slot.is_contiguous() && pos.numel() == qkv.size(0) &&
+                  slot.numel() == qkv.size(0), "pos and slot [T]");
+  TORCH_CHECK(q_out.is_contiguous() && q_out.dim() == 3 && q_out.size(0) == qkv.size(0) && q_out.size(1) == Hq &&
+                  q_out.size(2) == D && reinterpret_cast<uintptr_t>(q_out.data_ptr()) % 16 == 0,
+              "q_out [T, Hq, D], contiguous");
+  for (const auto* w : {&q_norm, &k_norm})
+    if (w->has_value()) {
+      req(**w, at::kBFloat16, "norm weight");
+      TORCH_CHECK((*w)->is_contiguous() && (*w)->numel() == D &&
+                      reinterpret_cast<uintptr_t>((*w)->data_ptr()) % 16 == 0, "norm weight [D]");
+    }
+  iob::BlockAppendArgs a{};
+  a.qkv = qkv.data_ptr();
+  a.qkv_stride = qkv.stride(0);
+  a.q_norm = q_norm.has_value() ? q_norm->data_ptr() : nullptr;
+  a.k_norm = k_norm.has_value() ? k_norm->data_ptr() : nullptr;
+  a.cos_sin = cos_sin.data_ptr<float>();
+  a.pos = pos.data_ptr<int>();
+  a.slot = slot.data_ptr<int>();
+  a.q_out = q_out.data_ptr();
+  a.pool = pool.data_ptr<uint8_t>();
+  a.codes = reinterpret_cast<int8_t*>(codes.data_ptr());
+  a.scale = scale.data_ptr();
+  a.fmt = static_cast<int>(fmt);
+  a.k_scale = static_cast<float>(k_scale);
+  a.v_scale = static_cast<float>(v_scale);
+  a.T = static_cast<int>(qkv.size(0));
+  a.Hq = static_cast<int>(Hq);
+  a.Hk = static_cast<int>(Hk);
+  a.D = static_cast<int>(D);
+  a.slots = static_cast<int>(pool.size(0) * 64);
+  a.max_pos = static_cast<int>(cos_sin.size(0));
+  a.eps = static_cast<float>(eps);
+  a.plus_one = plus_one;
+  const at::cuda::CUDAGuard g(qkv.device());
+  CHECK_CUDA_OK(iob::block_append(a, stream()));
+}
+
+void block_summarize(const at::Tensor& pool, const at::Tensor& pages, at::Tensor codes, at::Tensor scale, int64_t fmt,
+                     double k_scale, int64_t Hk, int64_t D) {
+  block_pool(pool, fmt, Hk, D);
+  block_bounds(codes, scale, pool.size(0), Hk, D);
+  req(pages, at::kInt, "pages");
+  TORCH_CHECK(pages.dim() == 1 && pages.is_contiguous(), "pages [n]");
+  iob::BlockAppendArgs a{};
+  a.pool = pool.data_ptr<uint8_t>();
+  a.codes = reinterpret_cast<int8_t*>(codes.data_ptr());
+  a.scale = scale.data_ptr();
+  a.fmt = static_cast<int>(fmt);
+  a.k_scale = static_cast<float>(k_scale);
+  a.Hk = static_cast<int>(Hk);
+  a.D = static_cast<int>(D);
+  a.slots = static_cast<int>(pool.size(0) * 64);
+  const at::cuda::CUDAGuard g(pool.device());
+  CHECK_CUDA_OK(iob::block_summarize(a, pages.data_ptr<int>(), static_cast<int>(pages.size(0)), stream()));
+}
+
+void block_select(const at::Tensor& q, const at::Tensor& codes, const at::Tensor& scale, const at::Tensor& page_table,
+                  c10::optional<at::Tensor> req_idx, const at::Tensor& kv_len, at::Tensor blocks, at::Tensor count,
+                  int64_t n_q, int64_t Hk, int64_t budget, int64_t sink, int64_t local) {
+  block_groups(q, page_table, req_idx, kv_len, n_q, Hk);
+  const int64_t D = q.size(2), B = kv_len.size(0);
+  TORCH_CHECK(D == 128 || D == 256 || D == 512, "head_dim 128, 256 or 512, got ", num(D));
+  block_bounds(codes, scale, codes.dim() > 0 ? codes.size(0) : 0, Hk, D);
+  req(blocks, at::kInt, "blocks");
+  req(count, at::kInt, "count");
+  TORCH_CHECK(sink >= 0 && local >= 1 && budget >= sink + local + 1 && budget <= iob::kBlockMaxList,
+              "budget must hold sink + local + 1 pages and at most ", num(iob::kBlockMaxList));
+  TORCH_CHECK(blocks.is_contiguous() && blocks.dim() == 3 && blocks.size(0) == B && blocks.size(1) == Hk &&
+                  blocks.size(2) == budget, "blocks [B, Hk, budget]");
+  TORCH_CHECK(count.is_contiguous() && count.dim() == 2 && count.size(0) == B && count.size(1) == Hk, "count [B, Hk]");
+  TORCH_CHECK(page_table.size(1) <= iob::kBlockSelectMaxPages, "page_table wider than ", num(iob::kBlockSelectMaxPages));
+  iob::BlockSelectArgs a{};
+  a.q = q.data_ptr();
+  a.q_stride = q.stride(0);
+  a.codes = reinterpret_cast<const int8_t*>(codes.data_ptr());
+  a.scale = scale.data_ptr();
+  a.page_table = page_table.data_ptr<int>();
+  a.req_idx = req_idx.has_value() ? req_idx->data_ptr<int>() : nullptr;
+  a.kv_len = kv_len.data_ptr<int>();
+  a.blocks = blocks.data_ptr<int>();
+  a.count = count.data_ptr<int>();
+  a.B = static_cast<int>(B);
+  a.n_q = static_cast<int>(n_q);
+  a.Hq = static_cast<int>(q.size(1));
+  a.Hk = static_cast<int>(Hk);
+  a.D = static_cast<int>(D);
+  a.rows = static_cast<int>(page_table.size(0));
+  a.pt_stride = static_cast<int>(page_table.size(1));
+  a.pages = static_cast<int>(codes.size(0));
+  a.budget = static_cast<int>(budget);
+  a.sink = static_cast<int>(sink);
+  a.local = static_cast<int>(local);
+  const at::cuda::CUDAGuard g(q.device());
+  CHECK_CUDA_OK(iob::block_select(a, stream()));
+}
+
+void block_decode(const at::Tensor& q, const at::Tensor& pool, const at::Tensor& page_table,
+                  c10::optional<at::Tensor> req_idx, const at::Tensor& kv_len, const at::Tensor& blocks, at::Tensor out,
+                  at::Tensor lse, c10::optional<at::Tensor> status, int64_t n_q, int64_t Hk, int64_t fmt,
+                  double sm_scale, double k_scale, double v_scale) {
+  block_groups(q, page_table, req_idx, kv_len, n_q, Hk);
+  const int64_t D = q.size(2), B = kv_len.size(0);
+  block_pool(pool, fmt, Hk, D);
+  req(blocks, at::kInt, "blocks");
+  req(out, at::kBFloat16, "out");
+  req(lse, at::kFloat, "lse");
+  TORCH_CHECK(blocks.is_contiguous() && blocks.dim() == 3 && blocks.size(0) == B && blocks.size(1) == Hk &&
+                  blocks.size(2) >= 1 && blocks.size(2) <= iob::kBlockMaxList, "blocks [B, Hk, 1 .. ",
+              num(iob::kBlockMaxList), "], contiguous");
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() &&
+                  reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0, "out like q, contiguous");
+  TORCH_CHECK(lse.is_contiguous() && lse.dim() == 2 && lse.size(0) == q.size(0) && lse.size(1) == q.size(1),
+              "lse [B * n_q, Hq]");
+  iob::BlockDecodeArgs a{};
+  a.q = q.data_ptr();
+  a.q_stride = q.stride(0);
+  a.pool = pool.data_ptr<uint8_t>();
+  a.page_table = page_table.data_ptr<int>();
+  a.req_idx = req_idx.has_value() ? req_idx->data_ptr<int>() : nullptr;
+  a.kv_len = kv_len.data_ptr<int>();
+  a.blocks = blocks.data_ptr<int>();
+  a.out = out.data_ptr();
+  a.lse = lse.data_ptr<float>();
+  if (status.has_value()) {
+    req(*status, at::kInt, "status");
+    TORCH_CHECK(status->numel() >= 1, "status [1]");
+    a.status = status->data_ptr<int>();
+  }
+  a.B = static_cast<int>(B);
+  a.n_q = static_cast<int>(n_q);
+  a.Hq = static_cast<int>(q.size(1));
+  a.Hk = static_cast<int>(Hk);
+  a.D = static_cast<int>(D);
+  a.rows = static_cast<int>(page_table.size(0));
+  a.pt_stride = static_cast<int>(page_table.size(1));
+  a.pages = static_cast<int>(pool.size(0));
+  a.budget = static_cast<int>(blocks.size(2));
+  a.fmt = static_cast<int>(fmt);
+  a.sm_scale = static_cast<float>(sm_scale);
+  a.k_scale = static_cast<float>(k_scale);
+  a.v_scale = static_cast<float>(v_scale);
+  const at::cuda::CUDAGuard g(q.device());
+  CHECK_CUDA_OK(iob::block_decode(a, stream()));
+}
+
 void mla_decode(c10::optional<at::Tensor> q, at::Tensor q8, at::Tensor q_scale, const at::Tensor& pool,
                 const at::Tensor& idx, at::Tensor out, c10::optional<at::Tensor> lse, at::Tensor o_part,
                 at::Tensor lse_part, at::Tensor status, int64_t fmt, int64_t tiles_per_split, int64_t num_splits,
@@ -951,6 +1164,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("moe_combine", &moe_combine);
   m.def("rmsnorm_quant", &rmsnorm_quant);
   m.def("gqa_extend", &gqa_extend);
+  m.def("block_append", &block_append);
+  m.def("block_summarize", &block_summarize);
+  m.def("block_select", &block_select);
+  m.def("block_decode", &block_decode);
   m.def("act_quant", &act_quant);
   m.def("splitk_reduce", &splitk_reduce);
   m.def("ep_dispatch", &ep_dispatch);

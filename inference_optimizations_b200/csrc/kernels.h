@@ -345,6 +345,63 @@ struct DcpMergeArgs {
 };
 cudaError_t dcp_merge(const DcpMergeArgs& a, cudaStream_t s);
 
+// ---- block-sparse attention over the paged GQA pool (block_sparse.cu, attn_block_decode.cu)
+constexpr int kBlockSelectMaxPages = 49152;   // page-table width of the selection (its scores live in shared memory)
+constexpr int kBlockMaxList = 2048;           // pages of one list
+
+// QKV epilogue of a layer whose pages carry key bounds: as GqaPrepArgs, every value rounded once, plus the bound of
+// each page whose last row is written.  Rows of one page are adjacent and ascending within a call.
+struct BlockAppendArgs {
+  const void* qkv;      // bf16 [T, (Hq + 2 Hk) * D], row stride qkv_stride elements
+  int64_t qkv_stride;
+  const void* q_norm;   // bf16 [D] or null (no norm)
+  const void* k_norm;
+  const float* cos_sin; // fp32 [max_pos, D]
+  const int* pos;       // [T]; a row whose position is outside the table is not written, its q is zero
+  const int* slot;      // [T]; outside [0, slots) = do not write
+  void* q_out;          // bf16 [T, Hq, D]
+  uint8_t* pool;        // layer pool base: [num_pages, Hk, block_bytes]
+  int8_t* codes;        // [num_pages, Hk, 2 (centre, half width), D]
+  void* scale;          // bf16 [num_pages, Hk], powers of two; inf = a key was not finite
+  int fmt;
+  float k_scale, v_scale;
+  int T, Hq, Hk, D, slots, max_pos, slab;
+  float eps;
+  bool plus_one;
+};
+cudaError_t block_append(const BlockAppendArgs& a, cudaStream_t s);
+cudaError_t block_summarize(const BlockAppendArgs& a, const int* pages, int n, cudaStream_t s);
+
+struct BlockSelectArgs {
+  const void* q;           // bf16 [B * n_q, Hq, D], row stride q_stride elements
+  int64_t q_stride;
+  const int8_t* codes;     // [pages, Hk, 2, D]
+  const void* scale;       // bf16 [pages, Hk]
+  const int* page_table;   // [rows, pt_stride]
+  const int* req_idx;      // [B] page-table row of group b (null: row b)
+  const int* kv_len;       // [B] tokens in the pool, the group's n_q tokens included
+  int* blocks;             // [B, Hk, budget] logical pages, ascending, -1 behind them
+  int* count;              // [B, Hk]
+  int B, n_q, Hq, Hk, D, rows, pt_stride, pages, budget, sink, local;
+};
+cudaError_t block_select(const BlockSelectArgs& a, cudaStream_t s);
+
+struct BlockDecodeArgs {
+  const void* q;           // bf16 [B * n_q, Hq, D], row stride q_stride elements
+  int64_t q_stride;
+  const uint8_t* pool;     // [pages, Hk, 2 parts, part_bytes]
+  const int* page_table;   // [rows, pt_stride]
+  const int* req_idx;      // [B] or null
+  const int* kv_len;       // [B]
+  const int* blocks;       // [B, Hk, budget] logical pages, each at most once; entries outside the request are skipped
+  void* out;               // bf16 [B * n_q, Hq, D]
+  float* lse;              // fp32 [B * n_q, Hq], natural log of the softmax's sum; -inf where nothing is visible
+  int* status;             // or null
+  int B, n_q, Hq, Hk, D, rows, pt_stride, pages, budget, fmt;
+  float sm_scale, k_scale, v_scale;
+};
+cudaError_t block_decode(const BlockDecodeArgs& a, cudaStream_t s);
+
 // ---- expert-parallel exchange over peer memory (ep.cu)
 struct EpDispatchArgs {
   const long long* peers;     // [world] base address of every rank's symmetric buffer (device)

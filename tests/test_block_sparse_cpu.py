@@ -1,0 +1,141 @@
+"""Block-sparse attention oracles: the bounds hold, the selection follows its rules, full lists are dense attention,
+refusals."""
+import math
+
+import pytest
+import torch
+
+from inference_optimizations_b200.ops import attention as A
+from inference_optimizations_b200.ops import block_sparse as S
+from inference_optimizations_b200.ops import kvcache as K
+from inference_optimizations_b200.ops.basic import rope_table
+
+FMTS = (K.FMT_BF16, K.FMT_FP8, K.FMT_NVFP4)
+
+
+def session(fmt, n, d=128, hq=4, hk=2, seed=0, step=None, ks=0.5, vs=0.5):
+    """A request of n tokens appended `step` rows at a time: (last q, pool, table, codes, scale)."""
+    g = torch.Generator().manual_seed(seed)
+    if fmt == K.FMT_BF16:
+        ks = vs = 1.0
+    npg = (n + 63) // 64
+    pool = torch.zeros(npg + 1, hk, 2, K.part_bytes(fmt, d), dtype=torch.uint8)
+    codes, sc = S.alloc_bounds(npg + 1, hk, d, "cpu")
+    table = (torch.randperm(npg, generator=g) + 1)[None].int()
+    qkv = torch.randn(n, (hq + 2 * hk) * d, generator=g).to(torch.bfloat16)
+    cs = rope_table(n + 64, d, 10000.0)
+    qs = []
+    for lo in range(0, n, step or n):
+        pos = torch.arange(lo, min(n, lo + (step or n)), dtype=torch.int32)
+        slot = (table[0, (pos // 64).long()] * 64 + pos % 64).int()
+        qs.append(S.block_append(qkv[pos.long()], None, None, cs, pos, slot, pool, codes, sc, fmt, hq, hk, d, 1e-6,
+                                 True, ks, vs))
+    return torch.cat(qs), pool, table, codes, sc, ks, vs
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_append_writes_what_the_existing_writer_writes(fmt):
+    d, hq, hk, n = 128, 4, 2, 150
+    _, pool, table, _, _, ks, vs = session(fmt, n)
+    g = torch.Generator().manual_seed(0)
+    torch.randperm(3, generator=g)
+    qkv = torch.randn(n, (hq + 2 * hk) * d, generator=g).to(torch.bfloat16)
+    pos = torch.arange(n, dtype=torch.int32)
+    slot = (table[0, (pos // 64).long()] * 64 + pos % 64).int()
+    p2 = torch.zeros_like(pool)
+    K.gqa_prep(qkv, None, None, rope_table(n + 64, d, 10000.0), pos, slot, p2, fmt, hq, hk, d, 1e-6, True, ks, vs)
+    k1, v1 = K.gqa_pool_read_ref(pool, table[0], n, fmt, d, ks, vs)
+    k2, v2 = K.gqa_pool_read_ref(p2, table[0], n, fmt, d, ks, vs)
+    assert torch.equal(v1, v2)                              # values are bf16 already: the same single rounding
+    step = {K.FMT_BF16: 0.0, K.FMT_FP8: 2 ** -3, K.FMT_NVFP4: 0.5}[fmt]
+    # keys go through fp32 here and through bf16 there: equal, or one step apart at a rounding boundary
+    assert ((k1 - k2).abs() <= step * torch.maximum(k1.abs(), k2.abs()) + 2 ** -8).all()
+    assert (k1 != k2).float().mean() < 0.05
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("step", [1, 7, 64, 100])
+def test_bounds_do_not_depend_on_the_calls(fmt, step):
+    a, b = session(fmt, 200), session(fmt, 200, step=step)
+    for x, y in zip(a[:5], b[:5]):
+        assert torch.equal(x, y)
+    assert (a[4][a[2][0, :3].long()] > 0).all() and not a[4][a[2][0, 3].long()].any()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_scores_bound_every_key_of_the_page(fmt):
+    d, hk = 128, 2
+    q, pool, table, codes, sc, ks, vs = session(fmt, 320)
+    keys, _ = K.gqa_pool_read_ref(pool, table[0], 320, fmt, d, ks, vs)
+    rows = q[-1].float()
+    for j in range(5):
+        p = int(table[0, j])
+        for h in range(hk):
+            c = codes[p, h].double() * float(sc[p, h])
+            for r in rows[2 * h:2 * h + 2].double():
+                top = (keys[64 * j:64 * j + 64, h].double() @ r).max()
+                # a code is at most half a step off (one step where it was clamped)
+                assert (r * c[0] + r.abs() * c[1]).sum() + r.abs().sum() * 2 * float(sc[p, h]) >= top
+
+
+def test_select_rules():
+    d, hk, hq = 128, 1, 1
+    q, pool, table, codes, sc, *_ = session(K.FMT_BF16, 64 * 20 + 10, hq=hq, hk=hk)
+    kv = torch.tensor([64 * 20 + 10], dtype=torch.int32)
+    phys = table[0].long()
+    scores = torch.stack([(q[-1, 0].float() * codes[p, 0, 0] + q[-1, 0].float().abs() * codes[p, 0, 1]).sum() * sc[p, 0]
+                          for p in phys])
+    for budget, sink, local in ((3, 1, 1), (8, 0, 2), (10, 3, 1), (21, 1, 1), (64, 1, 1)):
+        blocks, count = S.block_select(q[-1:], codes, sc, table, kv, 1, hk, budget, sink, local)
+        got = [x for x in blocks[0, 0].tolist() if x >= 0]
+        assert len(got) == count.item() == min(21, budget) and got == sorted(got)
+        assert set(range(sink)) <= set(got) and set(range(21 - local, 21)) <= set(got)
+        rest = [x for x in range(sink, 21 - local) if x not in got]
+        mid = [x for x in got if sink <= x < 21 - local]
+        if rest and mid:                                  # (codes of q round by up to 2^-7 of a step each)
+            assert min(scores[mid]) >= max(scores[rest]) * 0.97
+    # a verify group whose tokens straddle two pages keeps both
+    q4 = q[-14:-10].contiguous()
+    blocks, _ = S.block_select(q4, codes, sc, table, torch.tensor([64 * 20 + 2], dtype=torch.int32), 4, hk, 3)
+    assert blocks[0, 0].tolist() == [0, 19, 20]
+    empty, count = S.block_select(q[-1:], codes, sc, table, torch.tensor([0], dtype=torch.int32), 1, hk, 4)
+    assert count.item() == 0 and (empty == -1).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_full_lists_are_dense_attention(fmt):
+    q, pool, table, codes, sc, ks, vs = session(fmt, 200)
+    kv = torch.tensor([200], dtype=torch.int32)
+    for n_q in (1, 4):
+        blocks, _ = S.block_select(q[-n_q:], codes, sc, table, kv, n_q, 2, 4)
+        out, lse = S.block_decode(q[-n_q:], pool, table, kv, blocks, n_q, 2, fmt, 0.1, ks, vs)
+        want = A.gqa_decode_ref(q[-n_q:], pool, table, kv, n_q, 2, fmt, 0.1, 0, ks, vs)
+        assert (out.float() - want).abs().max() <= want.abs().max() * 2 ** -8 + 1e-6
+        assert torch.isfinite(lse).all()
+
+
+def test_empty_groups_and_garbage_past_the_end():
+    q, pool, table, codes, sc, ks, vs = session(K.FMT_BF16, 70)
+    pool.view(torch.bfloat16).view(-1, 2, 2, 64, 128)[int(table[0, 1]), :, :, 6:] = math.nan
+    kv = torch.tensor([70, 0], dtype=torch.int32)
+    blocks = torch.full((2, 2, 3), -1, dtype=torch.int32)
+    blocks[0, :, 1:] = torch.tensor([1, 0])
+    out, lse = S.block_decode(torch.cat([q[-1:], q[:1]]), pool, table.repeat(2, 1), kv, blocks, 1, 2, 0, 0.1)
+    assert torch.isfinite(out).all() and not out[1].any()
+    assert torch.isfinite(lse[0]).all() and (lse[1] == -math.inf).all()
+
+
+def test_refusals():
+    q, pool, table, codes, sc, *_ = session(K.FMT_BF16, 70)
+    kv = torch.tensor([70], dtype=torch.int32)
+    for kw in (dict(budget=2), dict(budget=4, sink=-1), dict(budget=4, local=0), dict(budget=S.MAX_LIST + 1)):
+        with pytest.raises(RuntimeError):
+            S.block_select(q[-1:], codes, sc, table, kv, 1, 2, **kw)
+    with pytest.raises(RuntimeError):
+        S.block_select(q[-9:], codes, sc, table, kv, 9, 2, 4)              # 18 rows
+    with pytest.raises(RuntimeError):
+        S.block_decode(q[-1:], pool, table, kv, torch.zeros(1, 3, 4, dtype=torch.int32), 1, 2, 0, 0.1)
+    with pytest.raises(RuntimeError):
+        S.block_decode(q[-1:], pool, table, kv, torch.zeros(1, 2, 4, dtype=torch.int32), 1, 2, 1, 0.1)
+    with pytest.raises(RuntimeError):
+        S.block_summarize(pool, torch.tensor([1]), codes[:1], sc, 0, 2, 128)

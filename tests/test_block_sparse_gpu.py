@@ -1,0 +1,525 @@
+"""Block-sparse attention kernels against the 64-bit / exact oracles: every head dim and pool format, ragged and empty
+groups, garbage past a request's end, ties, strides, streams, graphs, offsets past 32 bits."""
+import math
+
+import pytest
+import torch
+
+from inference_optimizations_b200.ops import block_sparse as S
+from inference_optimizations_b200.ops import kvcache as K
+from inference_optimizations_b200.ops.basic import rope_table
+
+pytestmark = pytest.mark.gpu
+
+FMTS = {"bf16": K.FMT_BF16, "fp8": K.FMT_FP8, "nvfp4": K.FMT_NVFP4}
+
+
+def rand_pool(pages, hk, fmt, d, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    pool = torch.randint(0, 256, (pages, hk, 2, K.part_bytes(fmt, d)), generator=g, dtype=torch.uint8)
+    if fmt == K.FMT_BF16:
+        pool.view(torch.bfloat16).copy_(torch.randn(pages, hk, 2, K.PAGE * d, generator=g))
+    elif fmt == K.FMT_FP8:
+        pool &= 0xBF
+    else:
+        sc = pool[..., K.PAGE * d // 2:]
+        sc &= 0x0F
+        sc |= 0x28
+    return pool
+
+
+def scales(fmt):
+    return (1.0, 1.0) if fmt == K.FMT_BF16 else (0.75, 1.25)
+
+
+# ------------------------------------------------------------------------------------------------ append
+def append_case(kind, seed):
+    """(pos, slot, pages): rows as the engine packs them."""
+    g = torch.Generator().manual_seed(seed)
+    perm = torch.randperm(63, generator=g) + 1
+    pos, slot, at = [], [], 0
+    if kind == "decode":                                   # one row a request, some finish their page
+        for i, p in enumerate([63, 0, 127, 64, 5, 191, 62]):
+            pos.append(p)
+            slot.append(int(perm[i]) * 64 + p % 64)
+    elif kind == "one":
+        pos, slot = [63], [int(perm[0]) * 64 + 63]
+    else:                                                  # prefill segments over page boundaries, padded ends
+        for start, n in ((0, 64), (60, 9), (17, 47), (30, 200), (5, 1), (63, 66)):
+            used = perm[at:at + (start + n + 63) // 64 - start // 64]
+            at += len(used)
+            for p in range(start, start + n):
+                pos.append(p)
+                slot.append(int(used[p // 64 - start // 64]) * 64 + p % 64)
+            while len(pos) % 4:
+                pos.append(pos[-1] + 1)
+                slot.append(-1)
+    return torch.tensor(pos, dtype=torch.int32), torch.tensor(slot, dtype=torch.int32), 64
+
+
+@pytest.mark.parametrize("kind", ["one", "decode", "prefill"])
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("d,hq,hk,norm,plus_one", [(128, 8, 2, True, False), (256, 3, 3, False, True),
+                                                   (512, 6, 2, True, True)])
+def test_append(cuda, kind, fmt, d, hq, hk, norm, plus_one):
+    fmt = FMTS[fmt]
+    ks, vs = scales(fmt)
+    pos, slot, pages = append_case(kind, d)
+    t = pos.numel()
+    g = torch.Generator().manual_seed(1)
+    wide = torch.randn(t, (hq + 2 * hk) * d + 24, generator=g).to(torch.bfloat16)      # strided rows
+    qn, kn = ((torch.randn(2, d, generator=g) * 0.2 + (0 if plus_one else 1)).to(torch.bfloat16)) if norm else (None, None)
+    cs = rope_table(300, d, 10000.0)
+    pool = rand_pool(pages, hk, fmt, d, 3)
+    codes, sc = S.alloc_bounds(pages, hk, d, "cpu")
+    codes.fill_(7)
+    sc.fill_(3.0)
+    dev = [x.to(cuda) if x is not None else None for x in (wide, qn, kn, cs, pos, slot, pool, codes, sc)]
+    q = S.block_append(dev[0][:, :(hq + 2 * hk) * d], *dev[1:], fmt, hq, hk, d, 1e-6, plus_one, ks, vs)
+    p2, c2, s2 = pool.clone(), codes.clone(), sc.clone()
+    want = S.block_append(wide[:, :(hq + 2 * hk) * d], qn, kn, cs, pos, slot, p2, c2, s2, fmt, hq, hk, d, 1e-6,
+                          plus_one, ks, vs)
+    # q: both sides round an fp32 result (error below 2^-18 of the vector's size) to bf16 once
+    size = want.float().abs().amax(-1, keepdim=True)
+    assert ((q.cpu().float() - want.float()).abs() <= want.float().abs() * 2 ** -7 + size * 2 ** -17).all()
+    # pool: rows that were not written are as they were; written rows decode to the oracle's up to one step
+    got = dev[6].cpu()
+    touched = torch.zeros(pages, dtype=torch.bool)
+    touched[(slot[slot >= 0] // 64).long()] = True
+    assert torch.equal(got[~touched], pool[~touched])
+    step = {K.FMT_BF16: 2 ** -7, K.FMT_FP8: 2 ** -3 + 2 ** -6, K.FMT_NVFP4: 0.5}[fmt]
+    tab = torch.arange(pages)
+    for a, b in zip(K.gqa_pool_read_ref(got, tab, pages * 64, fmt, d, ks, vs),
+                    K.gqa_pool_read_ref(p2, tab, pages * 64, fmt, d, ks, vs)):
+        off = (a - b).abs()
+        assert (off <= step * torch.maximum(a.abs(), b.abs()) + 2 ** -9 * ks * (2 if fmt == K.FMT_NVFP4 else 1)).all()
+        assert (off > 0).float().mean() < 2e-3            # a step only where the value lies at a rounding boundary
+        keep = torch.ones(pages * 64, dtype=torch.bool)
+        keep[slot[slot >= 0].long()] = False
+        assert torch.equal(a[keep], b[keep])
+    # bounds: exactly those of the stored keys on finished pages, untouched elsewhere
+    done = (slot[(slot >= 0) & (slot % 64 == 63)] // 64).int()
+    S.block_summarize(got, done, codes, sc, fmt, hk, d, ks)
+    assert torch.equal(dev[7].cpu(), codes) and torch.equal(dev[8].cpu(), sc)
+    # and the separate kernel says the same
+    c3, s3 = S.alloc_bounds(pages, hk, d, cuda)
+    S.block_summarize(dev[6], done.to(cuda), c3, s3, fmt, hk, d, ks)
+    assert torch.equal(c3.cpu()[done.long()], codes[done.long()])
+    assert torch.equal(s3.cpu()[done.long()], sc[done.long()])
+
+
+def test_append_prefill_slabs_match_single_rows(cuda):
+    """A long call (slabs of rows a CTA) writes what row-by-row calls write."""
+    d, hq, hk, t = 128, 4, 2, 1000
+    fmt = K.FMT_FP8
+    qkv = torch.randn(t, (hq + 2 * hk) * d, device=cuda).to(torch.bfloat16)
+    cs = rope_table(1100, d, 10000.0, cuda)
+    pos = torch.arange(37, 37 + t, dtype=torch.int32, device=cuda)
+    pages = 20
+    table = (torch.randperm(pages - 1) + 1)[: (37 + t + 63) // 64].to(cuda)
+    slot = (table[(pos // 64).long()] * 64 + pos % 64).int()
+    res = []
+    for step in (t, 1, 13):
+        pool = torch.zeros(pages, hk, 2, K.part_bytes(fmt, d), dtype=torch.uint8, device=cuda)
+        codes, sc = S.alloc_bounds(pages, hk, d, cuda)
+        q = torch.cat([S.block_append(qkv[i:i + step], None, None, cs, pos[i:i + step].contiguous(),
+                                      slot[i:i + step].contiguous(), pool, codes, sc, fmt, hq, hk, d, 1e-6, True)
+                       for i in range(0, t, step)])
+        res.append((q, pool, codes, sc))
+    for r in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(res[0], r))
+
+
+def test_append_out_of_range_rows(cuda):
+    """Rows with a slot or a position outside the buffers are skipped, nothing else moves."""
+    d, hq, hk = 128, 2, 1
+    qkv = torch.randn(5, (hq + 2 * hk) * d, device=cuda).to(torch.bfloat16)
+    pool = torch.zeros(2, hk, 2, K.part_bytes(0, d), dtype=torch.uint8, device=cuda)
+    codes, sc = S.alloc_bounds(2, hk, d, cuda)
+    pos = torch.tensor([0, 1, 10 ** 6, -3, 2], dtype=torch.int32, device=cuda)
+    slot = torch.tensor([-1, 128, 65, 66, 67], dtype=torch.int32, device=cuda)
+    args = (None, None, rope_table(64, d, 10000.0, cuda), pos, slot)
+    q = S.block_append(qkv, *args, pool, codes, sc, 0, hq, hk, d, 1e-6, True)
+    cpu = [x.cpu() if torch.is_tensor(x) else x for x in args]
+    p2 = torch.zeros_like(pool, device="cpu")
+    q2 = S.block_append(qkv.cpu(), *cpu, p2, *S.alloc_bounds(2, hk, d, "cpu"), 0, hq, hk, d, 1e-6, True)
+    assert torch.equal(q.cpu()[2:4], torch.zeros(2, hq, d, dtype=torch.bfloat16))
+    assert torch.allclose(q.cpu().float(), q2.float(), atol=2 ** -6)
+    nz = lambda p: p.view(2, hk, 2, 64, -1).any(-1).nonzero().tolist()  # noqa: E731
+    assert nz(pool.cpu()) == nz(p2) and not codes.any()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), 3.0e38])
+def test_bounds_of_keys_that_are_not_finite(cuda, bad):
+    d, hk = 128, 2
+    pool = rand_pool(3, hk, K.FMT_BF16, d, 5)
+    pool.view(torch.bfloat16).view(3, hk, 2, 64, d)[1, 1, 0, 17, 3] = bad
+    if bad == 3.0e38:                                       # hi - lo overflows
+        pool.view(torch.bfloat16).view(3, hk, 2, 64, d)[1, 1, 0, 20, 3 ^ 8 * (17 ^ 20) & 127] = -bad
+    c1, s1 = S.alloc_bounds(3, hk, d, cuda)
+    c2, s2 = S.alloc_bounds(3, hk, d, "cpu")
+    pages = torch.tensor([1, 2, 99, -1], dtype=torch.int32)
+    S.block_summarize(pool.to(cuda), pages.to(cuda), c1, s1, K.FMT_BF16, hk, d)
+    S.block_summarize(pool, pages, c2, s2, K.FMT_BF16, hk, d)
+    assert torch.equal(c1.cpu(), c2) and torch.equal(s1.cpu(), s2)
+    assert bad == 3.0e38 or (s1[1, 1] == math.inf and not c1[1, 1].any())
+    assert torch.isfinite(s1[1, 0]) and torch.isfinite(s1[2]).all()
+
+
+# ------------------------------------------------------------------------------------------------ select
+def rand_bounds(pages, hk, d, seed, spread=20.0):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.empty(pages, hk, 2, d, dtype=torch.int8)
+    codes[:, :, 0] = (torch.randn(pages, hk, d, generator=g) * spread).round().clamp(-127, 127)
+    codes[:, :, 1] = torch.randint(0, 128, (pages, hk, d), generator=g)
+    return codes, torch.exp2(torch.randint(-9, -2, (pages, hk), generator=g).float()).to(torch.bfloat16)
+
+
+def run_select(cuda, q, codes, sc, table, kv_len, n_q, hk, budget, **kw):
+    dev = {k: v.to(cuda) if torch.is_tensor(v) else v for k, v in kw.items()}
+    got = S.block_select(q.to(cuda), codes.to(cuda), sc.to(cuda), table.to(cuda), kv_len.to(cuda), n_q, hk, budget, **dev)
+    want = S.block_select(q, codes, sc, table, kv_len, n_q, hk, budget, **kw)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+    return got
+
+
+@pytest.mark.parametrize("d,hq,hk,n_q", [(128, 8, 2, 1), (128, 8, 2, 4), (256, 9, 3, 5), (512, 4, 4, 1), (512, 16, 1, 1),
+                                         (128, 2, 2, 16)])
+@pytest.mark.parametrize("budget,sink,local", [(3, 1, 1), (17, 1, 1), (9, 0, 3), (64, 2, 2)])
+def test_select(cuda, d, hq, hk, n_q, budget, sink, local):
+    lens = [0, 1, n_q, 63, 64, 65, 640, 64 * budget, 64 * budget + 1, 64 * 40 + 2, 64 * 301 - 1, 64 * 301]
+    b, width = len(lens), 304
+    table = torch.stack([torch.randperm(400)[:width] for _ in range(b + 1)]).to(torch.int32)
+    codes, sc = rand_bounds(400, hk, d, d + n_q)
+    q = (torch.randn(b * n_q, hq, d) * 2).to(torch.bfloat16)
+    req = torch.randperm(b + 1)[:b].to(torch.int32)
+    run_select(cuda, q, codes, sc, table, torch.tensor(lens, dtype=torch.int32), n_q, hk, budget, sink=sink, local=local,
+               req_idx=req)
+
+
+def test_select_ties_and_special_pages(cuda):
+    d, hk, hq = 128, 2, 4
+    codes, sc = rand_bounds(200, hk, d, 0)
+    codes[:, 0] = codes[0, 0]                           # kv head 0: every page scores alike -> lowest pages
+    sc[:, 0] = 0.25
+    codes[50:60, 1], sc[50:60, 1] = 0, math.inf         # kv head 1: pages that are always taken
+    table = torch.arange(200, dtype=torch.int32)[None].repeat(5, 1)
+    table[2, 30:90] = 7777                              # not pages of the pool: last
+    table[2, 100] = -5
+    q = torch.randn(5, hq, d).to(torch.bfloat16)
+    q[1, 0] = math.nan                                  # a row that is not finite has no say
+    q[3] = math.inf
+    q[4] = 0
+    kv = torch.full((5,), 200 * 64 - 7, dtype=torch.int32)
+    for budget in (3, 12, 150):
+        blocks, _ = run_select(cuda, q, codes, sc, table, kv, 1, hk, budget)
+        assert blocks[0, 0].tolist() == list(range(budget - 1)) + [199]
+    q2 = torch.randn(5, hq, d).to(torch.bfloat16)[:, :, :]
+    run_select(cuda, q2, codes, sc, table, kv, 1, hk, 2 + 1, sink=0, local=2)
+
+
+def test_select_of_long_requests_strided_q(cuda):
+    """Thousands of pages; q is a view of a wider buffer."""
+    d, hk, hq, b = 128, 1, 4, 3
+    codes, sc = rand_bounds(9000, hk, d, 9, 12.0)
+    table = torch.stack([torch.randperm(9000) for _ in range(b)]).to(torch.int32)
+    wide = torch.randn(b, hq * d + 64).to(torch.bfloat16)
+    kv = torch.tensor([9000 * 64, 5003 * 64 + 11, 4097 * 64], dtype=torch.int32)
+    dev = wide.to(cuda)[:, :hq * d].unflatten(1, (hq, d))
+    q = wide[:, :hq * d].unflatten(1, (hq, d))
+    for budget in (32, 1000, 2048):
+        got = S.block_select(dev, codes.to(cuda), sc.to(cuda), table.to(cuda), kv.to(cuda), 1, hk, budget)
+        want = S.block_select(q, codes, sc, table, kv, 1, hk, budget)
+        assert torch.equal(got[0].cpu(), want[0])
+
+
+# ------------------------------------------------------------------------------------------------ attend
+def check_attend(got, lse, q, pool, table, kv, blocks, n_q, hk, fmt, sm, req=None):
+    """Element bounds: P is rounded to 16 bits (relative 2^-9 bf16, 2^-12 f16, at least as fine) and the output to
+    bf16 (2^-9); scores are fp32 sums of exact products, off by at most D 2^-23 of the sum of their sizes."""
+    ks, vs = scales(fmt)
+    pc, tc = pool.cpu(), table.cpu()
+    want, wlse = S.block_decode_ref(q.cpu(), pc, tc, kv.cpu(), blocks.cpu(), n_q, hk, fmt, sm, ks, vs,
+                                    None if req is None else req.cpu(), torch.float64)
+    mag, _ = S.block_decode_ref(q.cpu(), abs_values(pc, fmt, q.shape[2]), tc, kv.cpu(), blocks.cpu(), n_q, hk, fmt, sm,
+                                ks, vs, None if req is None else req.cpu(), torch.float64)
+    d = q.shape[2]
+    size = (q.cpu().double().pow(2).sum(-1).sqrt() * math.sqrt(d) * 3.0 * sm)            # bound of sum |q||k| scale
+    ds = size * d * 2.0 ** -23 + 2.0 ** -20
+    tol = want.abs() * 2 ** -8 + mag * (2 ** -8 + 2 * ds[..., None])
+    bad = (got.cpu().double() - want).abs() > tol + 1e-30
+    assert not bad.any(), ((got.cpu().double() - want).abs() / (tol + 1e-30)).max()
+    fin = torch.isfinite(wlse)
+    assert torch.equal(fin, torch.isfinite(lse.cpu())) and (lse.cpu()[~fin] == -math.inf).all()
+    assert ((lse.cpu().double() - wlse).abs()[fin] <= (ds + 2.0 ** -20 * (1 + wlse.abs()))[fin]).all()
+
+
+def abs_values(pool, fmt, d):
+    """The pool with |V| (keys as they are): the oracle then gives sum p |v|."""
+    p = pool.clone()
+    if fmt == K.FMT_BF16:
+        p.view(torch.bfloat16)[:, :, 1].abs_()
+    elif fmt == K.FMT_FP8:
+        p[:, :, 1] &= 0x7F
+    else:
+        p[:, :, 1, :K.PAGE * d // 2] &= 0x77
+    return p
+
+
+def attend_case(cuda, d, hq, hk, n_q, fmt, lens, budget, seed, garbage=True):
+    g = torch.Generator().manual_seed(seed)
+    per = [(x + 63) // 64 for x in lens]
+    total = sum(per) + 2
+    pool = rand_pool(total, hk, fmt, d, seed)
+    width = max(per) + 2
+    table = torch.zeros(len(lens), width, dtype=torch.int32)
+    perm = (torch.randperm(total - 1, generator=g) + 1).to(torch.int32)
+    at = 0
+    blocks = torch.full((len(lens), hk, budget), -1, dtype=torch.int32)
+    for i, (n, m) in enumerate(zip(lens, per)):
+        table[i, :m] = perm[at:at + m]
+        at += m
+        if garbage and n % 64:                            # NaN in everything past the request's end
+            last = pool[int(table[i, m - 1])]
+            rb = K.row_bytes(fmt, d)
+            last[:, :, (n % 64) * rb:64 * rb] = 0xFF
+            if fmt == K.FMT_NVFP4:
+                last[:, :, 64 * rb + (n % 64) * (d // 16):] = 0x7F
+        for h in range(hk):
+            if m:
+                pick = torch.randperm(m, generator=g)[:budget]
+                if m - 1 not in pick.tolist():
+                    pick[-1] = m - 1
+                blocks[i, h, :len(pick)] = pick[torch.randperm(len(pick), generator=g)].int()
+    q = (torch.randn(len(lens) * n_q, hq, d, generator=g) * 2).to(torch.bfloat16)
+    kv = torch.tensor(lens, dtype=torch.int32)
+    return [x.to(cuda) for x in (q, pool, table, kv, blocks)]
+
+
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("d", [128, 256, 512])
+@pytest.mark.parametrize("hq,hk,n_q", [(1, 1, 1), (8, 2, 1), (6, 2, 4), (15, 3, 3), (2, 2, 16), (16, 1, 1)])
+def test_decode(cuda, fmt, d, hq, hk, n_q):
+    fmt = FMTS[fmt]
+    lens = [0, 1, 2, 31, 32, 33, 63, 64, 65, 97, 128, 500, 1000]
+    q, pool, table, kv, blocks = attend_case(cuda, d, hq, hk, n_q, fmt, lens, 7, d + hq)
+    sm = 1 / math.sqrt(d)
+    out, lse = S.block_decode(q, pool, table, kv, blocks, n_q, hk, fmt, sm, *scales(fmt))
+    assert torch.isfinite(out).all()
+    check_attend(out, lse, q, pool, table, kv, blocks, n_q, hk, fmt, sm)
+    again = S.block_decode(q, pool, table, kv, blocks, n_q, hk, fmt, sm, *scales(fmt))
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+@pytest.mark.parametrize("fmt,d", [("bf16", 128), ("bf16", 512), ("fp8", 256), ("nvfp4", 512)])
+@pytest.mark.parametrize("budget", [1, 2, 3, 8, 33, 100])
+@pytest.mark.parametrize("b", [1, 3])
+def test_decode_splits(cuda, fmt, d, budget, b):
+    """Few groups: the list is split over a cluster; every length of a CTA's share, empty shares among them."""
+    fmt = FMTS[fmt]
+    lens = [64 * 110 - 13, 64 * 3, 70][:b]
+    q, pool, table, kv, blocks = attend_case(cuda, d, 4, 2, 2, fmt, lens, budget, budget)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out, lse = S.block_decode(q, pool, table, kv, blocks, 2, 2, fmt, d ** -0.5, *scales(fmt), status=status)
+    check_attend(out, lse, q, pool, table, kv, blocks, 2, 2, fmt, d ** -0.5)
+    assert status.item() == 0
+
+
+def test_decode_many_groups(cuda):
+    """More groups than SMs (no split)."""
+    lens = [(i * 37) % 600 for i in range(180)]
+    q, pool, table, kv, blocks = attend_case(cuda, 128, 4, 2, 1, K.FMT_FP8, lens, 5, 77)
+    out, lse = S.block_decode(q, pool, table, kv, blocks, 1, 2, K.FMT_FP8, 128 ** -0.5, *scales(K.FMT_FP8))
+    check_attend(out, lse, q, pool, table, kv, blocks, 1, 2, K.FMT_FP8, 128 ** -0.5)
+
+
+def test_decode_skips_entries_outside_the_request(cuda):
+    lens = [300, 300]
+    q, pool, table, kv, blocks = attend_case(cuda, 128, 4, 2, 1, 0, lens, 8, 3)
+    want = S.block_decode(q, pool, table, kv, blocks, 1, 2, 0, 0.1)
+    wild = torch.full((2, 2, 20), -1, dtype=torch.int32, device=cuda)
+    wild[:, :, 3:11] = blocks
+    wild[:, :, 0] = 5                                     # past the request (300 tokens: pages 0 .. 4)
+    wild[:, :, 1] = 10 ** 9
+    wild[:, :, 2] = -10 ** 9
+    got = S.block_decode(q, pool, table, kv, wild, 1, 2, 0, 0.1)
+    check_attend(got[0], got[1], q, pool, table, kv, wild, 1, 2, 0, 0.1)
+    assert (got[0].float() - want[0].float()).abs().max() < 0.05
+    table[1] = 10 ** 8                                    # no page of the pool
+    table[0, 0] = -1
+    out, lse = S.block_decode(q, pool, table, kv, blocks, 1, 2, 0, 0.1)
+    assert not out[1].any() and (lse[1] == -math.inf).all()
+    check_attend(out, lse, q, pool, table, kv, blocks, 1, 2, 0, 0.1)
+    req = torch.tensor([0, 9], dtype=torch.int32, device=cuda)       # no row of the table
+    out, lse = S.block_decode(q, pool, table, kv, blocks, 1, 2, 0, 0.1, req_idx=req)
+    assert not out[1].any()
+
+
+def test_decode_large_and_small_queries(cuda):
+    """8-bit and 4-bit pools take queries through f16: sizes far outside its range, and rows of zeros, are exact in
+    scale (the softmax scale brings the scores back)."""
+    for fmt in (K.FMT_FP8, K.FMT_NVFP4):
+        q, pool, table, kv, blocks = attend_case(cuda, 128, 4, 2, 1, fmt, [300, 200], 5, 11)
+        for f in (2.0 ** 40, 2.0 ** -40):
+            big = (q.float() * f).to(torch.bfloat16)
+            out, lse = S.block_decode(big, pool, table, kv, blocks, 1, 2, fmt, 0.1 / f, *scales(fmt))
+            ref, rl = S.block_decode(q, pool, table, kv, blocks, 1, 2, fmt, 0.1, *scales(fmt))
+            assert torch.equal(out, ref) and torch.allclose(lse, rl, atol=1e-5)
+        q[0] = 0
+        out, lse = S.block_decode(q, pool, table, kv, blocks, 1, 2, fmt, 0.1, *scales(fmt))
+        check_attend(out, lse, q, pool, table, kv, blocks, 1, 2, fmt, 0.1)
+
+
+def test_decode_nan_query_stays_in_its_row(cuda):
+    q, pool, table, kv, blocks = attend_case(cuda, 256, 4, 2, 2, K.FMT_FP8, [300, 200], 4, 12)
+    ref, _ = S.block_decode(q, pool, table, kv, blocks, 2, 2, K.FMT_FP8, 0.05, *scales(K.FMT_FP8))
+    q[1, 2, 5] = math.nan
+    out, _ = S.block_decode(q, pool, table, kv, blocks, 2, 2, K.FMT_FP8, 0.05, *scales(K.FMT_FP8))
+    assert torch.isnan(out[1, 2]).all()
+    keep = torch.ones(4, 4, dtype=torch.bool)
+    keep[1, 2] = False
+    assert torch.equal(out[keep.to(cuda)], ref[keep.to(cuda)])
+
+
+def test_decode_strided_q_on_another_stream(cuda):
+    d, hq, hk = 128, 4, 2
+    q, pool, table, kv, blocks = attend_case(cuda, d, hq, hk, 1, 0, [1000, 77, 640], 6, 13)
+    want = S.block_decode(q, pool, table, kv, blocks, 1, hk, 0, 0.1)
+    wide = torch.zeros(3, hq * d + 40, dtype=torch.bfloat16, device=cuda)
+    wide[:, :hq * d] = q.flatten(1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = S.block_decode(wide[:, :hq * d].unflatten(1, (hq, d)), pool, table, kv, blocks, 1, hk, 0, 0.1)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_offsets_past_32_bits(cuda):
+    """A cache of more than 2^32 bytes and bounds of more than 2^31: the last pages are as good as the first."""
+    d, hk, hq = 512, 16, 16
+    pages = 2100                                           # x 2 MB
+    pool = torch.empty(pages, hk, 2, K.part_bytes(0, d), dtype=torch.uint8, device=cuda)
+    pool[-8:].view(torch.bfloat16).normal_()
+    pool[:8] = pool[-8:]
+    q = torch.randn(1, hq, d, device=cuda).to(torch.bfloat16)
+    kv = torch.tensor([8 * 64 - 5], dtype=torch.int32, device=cuda)
+    blocks = torch.arange(8, dtype=torch.int32, device=cuda).expand(1, hk, 8).contiguous()
+    lo = torch.arange(8, dtype=torch.int32, device=cuda)[None]
+    hi = lo + pages - 8
+    a = S.block_decode(q, pool, lo, kv, blocks, 1, hk, 0, 0.05)
+    b = S.block_decode(q, pool, hi, kv, blocks, 1, hk, 0, 0.05)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    cs = rope_table(600, d, 10000.0, cuda)
+    qkv = torch.randn(64, (hq + 2 * hk) * d, device=cuda).to(torch.bfloat16)
+    pos = torch.arange(64, dtype=torch.int32, device=cuda)
+    codes, sc = S.alloc_bounds(pages, hk, d, cuda)
+    for p in (3, pages - 1):
+        S.block_append(qkv, None, None, cs, pos, pos + p * 64, pool, codes, sc, 0, hq, hk, d, 1e-6, True)
+    assert torch.equal(pool[3], pool[-1]) and torch.equal(codes[3], codes[-1]) and torch.equal(sc[3], sc[-1])
+    assert codes[3].any()
+    del pool
+    pages = (1 << 31) // (hk * 2 * d) + 50
+    codes, sc = S.alloc_bounds(pages, hk, d, cuda)
+    codes[-40:] = torch.randint(-127, 128, (40, hk, 2, d), device=cuda, dtype=torch.int8)
+    codes[-40:, :, 1].abs_()
+    sc[-40:] = 0.5
+    codes[:40], sc[:40] = codes[-40:], sc[-40:]
+    kv = torch.tensor([40 * 64], dtype=torch.int32, device=cuda)
+    lo = torch.arange(40, dtype=torch.int32, device=cuda)[None]
+    a = S.block_select(q, codes, sc, lo, kv, 1, hk, 9)
+    b = S.block_select(q, codes, sc, lo + pages - 40, kv, 1, hk, 9)
+    assert torch.equal(a[0], b[0]) and len({tuple(x) for x in a[0][0].tolist()}) > 1
+
+
+# ------------------------------------------------------------------------------------------------ together
+@pytest.mark.parametrize("fmt", list(FMTS))
+def test_pipeline_with_room_for_every_page_is_dense_attention(cuda, fmt):
+    from inference_optimizations_b200.ops import attention as A
+    fmt = FMTS[fmt]
+    ks, vs = scales(fmt)
+    d, hq, hk, n = 256, 8, 4, 500
+    pages = 12
+    pool = torch.zeros(pages, hk, 2, K.part_bytes(fmt, d), dtype=torch.uint8, device=cuda)
+    codes, sc = S.alloc_bounds(pages, hk, d, cuda)
+    cs = rope_table(600, d, 10000.0, cuda)
+    pos = torch.arange(n, dtype=torch.int32, device=cuda)
+    table = (torch.randperm(pages - 1, device=cuda) + 1)[None].int()
+    slot = (table[0][(pos // 64).long()] * 64 + pos % 64).int()
+    qkv = torch.randn(n, (hq + 2 * hk) * d, device=cuda).to(torch.bfloat16)
+    q = S.block_append(qkv, None, None, cs, pos, slot, pool, codes, sc, fmt, hq, hk, d, 1e-6, True, ks, vs)[-1:]
+    kv = torch.tensor([n], dtype=torch.int32, device=cuda)
+    blocks, count = S.block_select(q, codes, sc, table, kv, 1, hk, 8)
+    assert (count == 8).all() and torch.equal(blocks[0, 0].cpu(), torch.arange(8, dtype=torch.int32))
+    out, _ = S.block_decode(q, pool, table, kv, blocks, 1, hk, fmt, d ** -0.5, ks, vs)
+    want = A.gqa_decode_ref(q.cpu(), pool.cpu(), table.cpu(), kv.cpu(), 1, hk, fmt, d ** -0.5, 0, ks, vs)
+    assert (out.cpu().float() - want).abs().max() < 2 ** -7 * want.abs().max()
+
+
+def test_pipeline_in_a_cuda_graph(cuda):
+    """Fixed addresses, lengths that change between replays."""
+    d, hq, hk, fmt, budget = 128, 8, 2, K.FMT_NVFP4, 6
+    q, pool, table, kv, _ = attend_case(cuda, d, hq, hk, 1, fmt, [1500, 900], 4, 21, garbage=False)
+    codes, sc = S.alloc_bounds(pool.shape[0], hk, d, cuda)
+    S.block_summarize(pool, torch.arange(pool.shape[0], dtype=torch.int32, device=cuda), codes, sc, fmt, hk, d)
+    cs = rope_table(2000, d, 10000.0, cuda)
+    qkv = torch.randn(2, (hq + 2 * hk) * d, device=cuda).to(torch.bfloat16)
+    pos, slot = kv - 1, torch.zeros(2, dtype=torch.int32, device=cuda)
+
+    def step():
+        p = kv - 1
+        pos.copy_(p)
+        slot.copy_(table.gather(1, (p // 64).long()[:, None])[:, 0] * 64 + p % 64)
+        qq = S.block_append(qkv, None, None, cs, pos, slot, pool, codes, sc, fmt, hq, hk, d, 1e-6, True)
+        blocks, _ = S.block_select(qq, codes, sc, table, kv, 1, hk, budget)
+        return S.block_decode(qq, pool, table, kv, blocks, 1, hk, fmt, 0.1)
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = step()
+    for lens in ([1500, 900], [1408, 64], [3, 832]):
+        kv.copy_(torch.tensor(lens, dtype=torch.int32))
+        g.replay()
+        got = [x.clone() for x in res]
+        want = step()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_refusals(cuda):
+    d, hq, hk = 128, 8, 2
+    q, pool, table, kv, blocks = attend_case(cuda, d, hq, hk, 1, 0, [200, 100], 4, 1)
+    codes, sc = S.alloc_bounds(pool.shape[0], hk, d, cuda)
+    ok = lambda **k: S.block_decode(**{**dict(q=q, pool=pool, page_table=table, kv_len=kv, blocks=blocks, n_q=1, hk=hk,  # noqa: E731
+                                              fmt=0, sm_scale=0.1), **k})
+    ok()
+    for k in (dict(q=q.float()), dict(q=q[..., :64]), dict(q=q[:1]), dict(n_q=2), dict(hk=3), dict(fmt=1), dict(fmt=9),
+              dict(pool=pool[:, :1]), dict(kv_len=kv.long()), dict(blocks=blocks.long()), dict(blocks=blocks[:, :, ::2]),
+              dict(blocks=blocks[:1]), dict(page_table=table.long()), dict(page_table=table[:1]),
+              dict(req_idx=torch.zeros(5, dtype=torch.int32, device=cuda)), dict(q=q.transpose(1, 2)),
+              dict(blocks=torch.zeros(2, hk, S.MAX_LIST + 1, dtype=torch.int32, device=cuda)), dict(pool=pool.cpu()),
+              dict(out=torch.empty(1, hq, d, dtype=torch.bfloat16, device=cuda))):
+        with pytest.raises(RuntimeError):
+            ok(**k)
+    sel = lambda **k: S.block_select(**{**dict(q=q, codes=codes, scale=sc, page_table=table, kv_len=kv, n_q=1, hk=hk,  # noqa: E731
+                                               budget=4), **k})
+    sel()
+    for k in (dict(budget=2), dict(budget=S.MAX_LIST + 1), dict(local=0), dict(sink=-1), dict(sink=3), dict(codes=codes[:, :1]),
+              dict(codes=codes.view(torch.uint8)), dict(scale=sc.float()), dict(n_q=16),
+              dict(page_table=torch.zeros(2, S.MAX_PAGES + 1, dtype=torch.int32, device=cuda))):
+        with pytest.raises(RuntimeError):
+            sel(**k)
+    qkv = torch.zeros(2, (hq + 2 * hk) * d, dtype=torch.bfloat16, device=cuda)
+    i2 = torch.zeros(2, dtype=torch.int32, device=cuda)
+    cs = rope_table(64, d, 1e4, cuda)
+    app = lambda **k: S.block_append(**{**dict(qkv=qkv, q_norm=None, k_norm=None, cos_sin=cs, pos=i2, slot=i2 - 1,  # noqa: E731
+                                               pool=pool, codes=codes, scale=sc, fmt=0, hq=hq, hk=hk, d=d, eps=1e-6,
+                                               plus_one=True), **k})
+    app()
+    for k in (dict(qkv=qkv.float()), dict(qkv=qkv[:, 8:]), dict(pos=i2.long()), dict(slot=i2[:1]), dict(cos_sin=cs[:, :64]),
+              dict(fmt=2), dict(d=64), dict(codes=codes[:1]), dict(q_norm=cs[0]), dict(hk=4)):
+        with pytest.raises(RuntimeError):
+            app(**k)
+    with pytest.raises(RuntimeError):
+        S.block_summarize(pool, i2.long(), codes, sc, 0, hk, d)
