@@ -220,6 +220,12 @@ class EngineConfig:
                                          # prefix cache also keeps each request's recurrent state at page
                                          # boundaries, stored in that row format, and restores it on a match
     kda_state_cache_max: int = 64        # recurrent-state snapshots the prefix cache keeps (least recent dropped)
+    # block-sparse decode (GQA family, `ops/block_sparse.py`): on global layers each decode / verify group attends to
+    # at most this many 64-token pages per kv head, ranked by 8-bit bounds of their keys; 0 = every page.  Prefill is
+    # dense.  The first `sparse_sink` pages and the last `sparse_local` are always among them.
+    sparse_pages: int = 0
+    sparse_sink: int = 1
+    sparse_local: int = 1
     # runtime
     cuda_graphs: bool = True
     extend_kernel: bool = True           # GQA prefill over NVFP4 / FP8 pools through the 128-row extend kernel

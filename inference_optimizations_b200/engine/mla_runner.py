@@ -139,6 +139,9 @@ class MLARunner:
         # reaches a page boundary, the latest snapshot goes to the prefix's radix node when the request leaves, and
         # a match is cut back to the deepest node holding a state, which is restored into the new request's row).
         # kvmix pools do not reuse prefixes (a promotion would move pages other requests share).
+        if ecfg.sparse_pages:
+            raise ValueError("sparse_pages (block-sparse decode over K / V pages) is a GQA-family option; the MLA "
+                             "family selects tokens with its indexer")
         self.state_fmt = ecfg.kda_state_cache if cfg.kda_every else ""
         if self.state_fmt not in ("", "fp32", "bf16", "fp8"):
             raise ValueError(f"kda_state_cache keeps fp32, bf16 or fp8 state rows, not {self.state_fmt!r}")

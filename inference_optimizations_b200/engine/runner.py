@@ -86,6 +86,16 @@ class GQARunner:
                  global_pages: Optional[int] = None):
         if ecfg.kv_dtype == "kvmix":
             raise ValueError("kv_dtype 'kvmix' (FP8 + NVFP4 latent rows in one page space) is an MLA-family pool")
+        sparse = None
+        if ecfg.sparse_pages:
+            from ..ops.block_sparse import HEAD_DIMS, MAX_LIST
+            sparse = (ecfg.sparse_pages, ecfg.sparse_sink, ecfg.sparse_local)
+            rows = (4 if ecfg.spec else 1) * (cfg.num_q_heads // cfg.num_kv_heads_global)
+            if not (sparse[1] >= 0 and sparse[2] >= 1 and sparse[1] + sparse[2] + 1 <= sparse[0] <= MAX_LIST):
+                raise ValueError(f"sparse_pages holds sparse_sink + sparse_local + 1 to {MAX_LIST} pages")
+            if cfg.head_dim_global not in HEAD_DIMS or rows > 16:
+                raise ValueError(f"block-sparse decode needs global head_dim in {HEAD_DIMS} and at most 16 query rows "
+                                 f"per kv head (verify tokens x group), got {cfg.head_dim_global}, {rows}")
         self.cfg, self.ecfg, self.device = cfg, ecfg, torch.device(device)
         self.tp, self.tp_rank = tp, tp_rank
         self.max_seq = max_seq
@@ -135,10 +145,12 @@ class GQARunner:
             fmt = K.FMT_IDS[ecfg.kv_dtype]
             n_glob = sum(1 for i in range(cfg.num_layers) if cfg.is_global(i))
             page_bytes = n_glob * (cfg.num_kv_heads_global // tp) * 2 * K.part_bytes(fmt, cfg.head_dim_global)
+            if sparse:                                   # the pages' key bounds
+                page_bytes += n_glob * (cfg.num_kv_heads_global // tp) * (2 * cfg.head_dim_global + 2)
             global_pages = pool_pages(ecfg, self.max_running * ((max_seq + 64 + 63) // 64) + 2, page_bytes, device)
         self.pool_tokens = 64 * (global_pages - 2)
         self.kv = GQAKVCache(cfg, tp, device, ecfg.kv_dtype, self.max_running + 1, max_seq + 64, global_pages,
-                             swa_pages, draft_pages=swa_pages if self.spec else 0)
+                             swa_pages, draft_pages=swa_pages if self.spec else 0, sparse=sparse)
         self.dummy_row = self.max_running
         self.pages: dict[int, dict[str, RequestPages]] = {}
         max_tok = max(ecfg.chunked_prefill + 16 * self.n_q_prefill, self.max_running * (self.n_draft + 1))
@@ -466,6 +478,7 @@ class GQARunner:
 
     def _decode_body(self, bucket: int) -> Callable:
         st = self.stage.step_tensors(bucket, bucket, 1, self._splits(bucket))
+        st.sparse = True
 
         def body():
             x, resid = self._target(st)
@@ -581,6 +594,7 @@ class GQARunner:
         st_d2 = self.st_d2.step_tensors(bucket, bucket, 1, sp)
         st_d3 = self.st_d3.step_tensors(bucket, bucket, 1, sp)
         st_ver = self.st_ver.step_tensors(bucket * 4, bucket, 4, sp)
+        st_ver.sparse = True
         h = self.cfg.hidden
         rows = torch.arange(bucket, device=self.device) * 4
         d_tok = torch.zeros(3, bucket, dtype=torch.int32, device=self.device)

@@ -61,6 +61,7 @@ def synth_decode_sessions(engine, n: int, ctx: int, max_new: int, seed: int = 0)
     for i, (pool, kind) in enumerate(zip(runner.kv.pools, runner.kv.kinds)):
         d = engine.cfg.head_dim_global if kind == "global" else engine.cfg.head_dim
         fill_pool_random(pool, runner.kv.fmt, d, seed * 7919 + i)
+    runner.kv.summarize()
     if hasattr(runner, "after_synthetic"):
         runner.after_synthetic(reqs)
     return reqs

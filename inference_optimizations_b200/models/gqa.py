@@ -32,6 +32,7 @@ import torch.nn.functional as Fn
 from ..config import GQAConfig
 from ..ops import attention as A
 from ..ops import basic as B
+from ..ops import block_sparse as S
 from ..ops import kvcache as K
 from ..ops import linear as L
 
@@ -224,9 +225,22 @@ class GQAModel:
         cs = self.rope_table(g.head_dim, theta, kv.max_pos)
         pool = kv.pools[layer_id]
         slot = st.slot[g.kind]
-        q = K.gqa_prep(qkv, w.q_norm if cfg.qk_norm else None, w.k_norm if cfg.qk_norm else None, cs, st.pos, slot,
-                       pool, kv.fmt, g.q_heads, g.kv_heads, g.head_dim, eps, True, kv.k_scale, kv.v_scale)
-        if st.ext_segs is not None and kv.fmt != K.FMT_BF16 and g.head_dim in (256, 512) and q.is_cuda:
+        q_norm, k_norm = (w.q_norm, w.k_norm) if cfg.qk_norm else (None, None)
+        bounds = kv.bounds[layer_id] if kv.bounds else None
+        if bounds is not None:
+            q = S.block_append(qkv, q_norm, k_norm, cs, st.pos, slot, pool, *bounds, kv.fmt, g.q_heads, g.kv_heads,
+                               g.head_dim, eps, True, kv.k_scale, kv.v_scale)
+        else:
+            q = K.gqa_prep(qkv, q_norm, k_norm, cs, st.pos, slot, pool, kv.fmt, g.q_heads, g.kv_heads, g.head_dim,
+                           eps, True, kv.k_scale, kv.v_scale)
+        if bounds is not None and st.sparse:
+            pages, sink, local = kv.sparse
+            table = kv.tables[g.kind].dev
+            blocks, _ = S.block_select(q, *bounds, table, st.kv_len, st.n_q, g.kv_heads, pages, sink, local, st.req_idx)
+            attn, _ = S.block_decode(q, pool, table, st.kv_len, blocks, st.n_q, g.kv_heads, kv.fmt,
+                                     1.0 / math.sqrt(g.head_dim), kv.k_scale, kv.v_scale, st.req_idx,
+                                     status=kv.sparse_status)
+        elif st.ext_segs is not None and kv.fmt != K.FMT_BF16 and g.head_dim in (256, 512) and q.is_cuda:
             attn = A.gqa_extend(q, pool, kv.tables[g.kind].dev, st.ext_blocks(g.q_heads // g.kv_heads, q.device),
                                 g.kv_heads, kv.fmt, 1.0 / math.sqrt(g.head_dim), g.window, kv.k_scale, kv.v_scale,
                                 status=kv.ext_status)
@@ -330,6 +344,7 @@ class StepTensors:
     # runs the GQA-packed extend kernel over NVFP4 / FP8 pools (block lists cached per group size G)
     ext_segs: Optional[list] = None
     ext_cache: dict = field(default_factory=dict)
+    sparse: bool = False              # global layers attend to the selected pages only (decode and verify steps)
     lane: int = 0                     # 1 = the prefill lane of the SM-partitioned lanes (its own decode workspace)
 
     def ext_blocks(self, g: int, device) -> torch.Tensor:
@@ -347,7 +362,9 @@ class GQAKVCache:
 
     def __init__(self, cfg: GQAConfig, tp: int, device, fmt: str, max_requests: int, max_seq: int,
                  global_pages: int, swa_pages: int, draft_pages: int = 0, k_scale: float = 1.0,
-                 v_scale: float = 1.0):
+                 v_scale: float = 1.0, sparse: Optional[tuple] = None):
+        """sparse = (pages, sink, local): the global layers' pools carry 8-bit key bounds per page and kv head
+        (`ops/block_sparse.py`) and decode steps attend to `pages` pages of them."""
         from ..kv.allocator import PageAllocator, PageTable
         self.cfg, self.fmt_name, self.fmt = cfg, fmt, K.FMT_IDS[fmt]
         self.device = torch.device(device)
@@ -356,6 +373,8 @@ class GQAKVCache:
         max_pages = (max_seq + 63) // 64 + 1
         self.pools = []
         self.kinds = []
+        self.sparse = sparse
+        self.bounds = []                 # per layer (codes, scale) of its pages, or None; empty without `sparse`
         for i in range(cfg.num_layers):
             glob = cfg.is_global(i)
             d = cfg.head_dim_global if glob else cfg.head_dim
@@ -363,11 +382,15 @@ class GQAKVCache:
             n = global_pages if glob else swa_pages
             self.pools.append(torch.zeros(n, hk, 2, K.part_bytes(self.fmt, d), dtype=torch.uint8, device=device))
             self.kinds.append("global" if glob else "swa")
+            if sparse:
+                self.bounds.append(S.alloc_bounds(n, hk, d, device) if glob else None)
         if draft_pages:
             for _ in range(cfg.draft_layers):
                 self.pools.append(torch.zeros(draft_pages, cfg.num_kv_heads // tp, 2, K.part_bytes(self.fmt, cfg.head_dim),
                                               dtype=torch.uint8, device=device))
                 self.kinds.append("draft")
+                if sparse:
+                    self.bounds.append(None)
         self.alloc = {"global": PageAllocator(global_pages), "swa": PageAllocator(swa_pages)}
         self.tables = {"global": PageTable(max_requests, max_pages, device), "swa": PageTable(max_requests, max_pages, device)}
         if draft_pages:
@@ -375,6 +398,7 @@ class GQAKVCache:
             self.tables["draft"] = PageTable(max_requests, max_pages, device)
         self._ws = {}
         self.ext_status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.sparse_status = torch.zeros(1, dtype=torch.int32, device=device)
 
     def workspace(self, d: int, hk: int, lane: int = 0) -> Optional[A.DecodeWorkspace]:
         """The decode lane's reserved split workspace; the prefill lane (lane 1) gets None, so each call allocates
@@ -392,6 +416,15 @@ class GQAKVCache:
             need = max_groups * hk * max_splits * 16
             if key not in self._ws or self._ws[key].lse_part.numel() < need:
                 self._ws[key] = A.DecodeWorkspace.allocate(max_groups, hk, max_splits, d, device=self.device)
+
+    def summarize(self) -> None:
+        """Key bounds of every page from the pools' contents: after something other than the model's own append wrote
+        them."""
+        for pool, b in zip(self.pools, self.bounds):
+            if b is not None:
+                codes, scale = b
+                S.block_summarize(pool, torch.arange(pool.shape[0], dtype=torch.int32, device=pool.device), codes,
+                                  scale, self.fmt, codes.shape[1], codes.shape[3], self.k_scale)
 
     def sync_tables(self) -> None:
         for t in self.tables.values():

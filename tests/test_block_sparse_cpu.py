@@ -136,3 +136,72 @@ def test_refusals():
         S.block_decode(q[-1:], pool, table, kv, torch.zeros(1, 2, 4, dtype=torch.int32), 1, 2, 1, 0.1)
     with pytest.raises(RuntimeError):
         S.block_summarize(pool, torch.tensor([1]), codes[:1], sc, 0, 2, 128)
+
+
+# ------------------------------------------------------------------------------------------------ engine
+def _engine(**kw):
+    from inference_optimizations_b200.config import EngineConfig
+    from inference_optimizations_b200.engine.engine import Engine
+    kw = {**dict(model="tiny_gqa", device="cpu", kv_dtype="bf16", max_running=4, chunked_prefill=100, cuda_graphs=False),
+          **kw}
+    return Engine(EngineConfig(**kw), max_seq=512)
+
+
+def _follows_reference(eng, prompts, outs, gap=1e-2):
+    n = 0
+    for p, o in zip(prompts, outs):
+        seq = list(p)
+        for tok in o:
+            ref = eng.runner.model.reference_logits(seq)[-1]
+            top = torch.topk(ref, 2).values
+            if (top[0] - top[1]).item() > gap:           # not a numerical tie
+                assert tok == int(ref.argmax())
+                n += 1
+            seq.append(tok)
+    return n
+
+
+@pytest.mark.parametrize("spec", [False, True])
+def test_engine_with_room_for_every_page_is_the_dense_engine(spec):
+    from inference_optimizations_b200.engine.scheduler import SamplingParams
+    torch.manual_seed(0)
+    eng = _engine(sparse_pages=8, spec=spec)
+    prompts = [torch.randint(1, 500, (n,)).tolist() for n in (190, 9, 130)]
+    outs = eng.generate(prompts, SamplingParams(max_new_tokens=6))
+    assert _follows_reference(eng, prompts, outs) >= 6
+
+
+def test_engine_attends_to_the_selected_pages(monkeypatch):
+    from inference_optimizations_b200.engine.scheduler import SamplingParams
+    torch.manual_seed(1)
+    eng = _engine(sparse_pages=3)
+    seen = []
+    real = S.block_select
+
+    def spy(*a, **k):
+        r = real(*a, **k)
+        seen.append((a[4].clone(), r[0].clone(), r[1].clone()))
+        return r
+    monkeypatch.setattr(S, "block_select", spy)
+    outs = eng.generate([torch.randint(1, 500, (450,)).tolist(), [7] * 20], SamplingParams(max_new_tokens=5))
+    assert all(len(o) == 5 for o in outs)
+    assert len(seen) >= 2 * 4                              # both global layers, every decode step
+    for kv, blocks, count in seen:
+        for b, n in enumerate(kv.tolist()):
+            npg = (n + 63) // 64
+            assert (count[b] == min(npg, 3)).all()
+            assert (blocks[b, :, min(npg, 3) - 1] == npg - 1).all() and (blocks[b, :, 0] == 0).all()
+    # every finished page of the requests had its bounds when it was ranked: recomputing them changes nothing
+    kv = eng.runner.kv
+    before = [(c.clone(), s.clone()) for c, s in (b for b in kv.bounds if b is not None)]
+    kv.summarize()
+    for (c, s), (c2, s2) in zip(before, (b for b in kv.bounds if b is not None)):
+        done = s.ne(0).all(1)
+        assert done.sum() >= 7 and torch.equal(c[done], c2[done]) and torch.equal(s[done], s2[done])
+
+
+def test_engine_refuses_what_it_cannot_serve():
+    for kw in (dict(sparse_pages=2), dict(sparse_pages=4000), dict(sparse_pages=4, sparse_local=0),
+               dict(sparse_pages=4, model="tiny_mla", kv_dtype="nvfp4")):
+        with pytest.raises(ValueError):
+            _engine(**kw)
