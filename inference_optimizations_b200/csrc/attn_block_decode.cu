@@ -33,7 +33,7 @@ struct Cfg {
   static constexpr int SC = FMT == kKvNvfp4 ? D / 16 : 0;  // scale bytes per row
   static constexpr int PART = TT * (RB + SC);              // one of K, V of a tile
   static constexpr int STAGE = 2 * PART;
-  static constexpr int NS = STAGE <= 20480 ? 4 : 3;
+  static constexpr int NS = STAGE <= 20480 ? 4 : FMT == kKvNvfp4 ? 2 : 3;
   static constexpr int NCH = RB / 16 < 8 ? RB / 16 : 8;    // chunk swizzle span of a row
   static constexpr int SST = TT + (DS == 1 ? 8 : 16);      // floats between score rows
   static constexpr int PST = TT + 8;                       // 16-bit values between P rows
@@ -45,6 +45,8 @@ struct Cfg {
   static constexpr int off_p = off_s + DS * kRows * SST * 4;
   static constexpr int off_list = off_p + kRows * PST * 2;
   static constexpr int smem(int cap) { return off_list + 8 * cap; }
+  // CTAs that share an SM: by shared memory, at most 4
+  static constexpr int RES = 230000 / (off_list + 3072) < 4 ? 230000 / (off_list + 3072) : 4;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -106,7 +108,7 @@ __device__ __forceinline__ uint32_t q_pair(const __nv_bfloat16* q, float f) {
 }
 
 template <class C>
-__global__ void __launch_bounds__(C::NT) block_decode_kernel(const BlockDecodeArgs a, const int csize, const int cap) {
+__global__ void __launch_bounds__(C::NT, C::RES) block_decode_kernel(const BlockDecodeArgs a, const int csize, const int cap) {
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ __align__(8) uint64_t full[C::NS];
   __shared__ float s_alpha[kRows], s_m[kRows], s_l[kRows], s_qf[kRows], s_f[8][kRows];
@@ -398,12 +400,12 @@ __global__ void __launch_bounds__(C::NT) block_decode_kernel(const BlockDecodeAr
                 const int t0 = kt * 32 + k * 8 + 2 * j4, blk = 2 * (c0 + c) + (lane >> 4);
                 const uint32_t sb = vsc[t0 * C::SC + blk] | (static_cast<uint32_t>(vsc[(t0 + 1) * C::SC + blk]) << 8);
                 const uint32_t s2 = e4m3x2_to_f16x2(static_cast<uint16_t>(sb));
-                // nibbles of tokens t0 (low half) and t0 + 1 (high half) -> bytes of one value's token pair
-                const uint32_t lo = r[k] & 0xffffu, hi = r[k] >> 16;
-                const uint32_t ev = (lo & 0x0f0fu) | ((hi & 0x0f0fu) << 4);            // values 0, 2
-                const uint32_t od = ((lo >> 4) & 0x0f0fu) | (hi & 0xf0f0u);            // values 1, 3
+                // nibbles of tokens t0 (low half) and t0 + 1 (high half) -> bytes of one value's token pair, in
+                // the low halves of two bit selections
+                const uint32_t ev = (r[k] & 0x0f0f0f0fu) | ((r[k] >> 12) & 0xf0f0f0f0u);       // values 0, 2
+                const uint32_t od = ((r[k] >> 4) & 0x0f0f0f0fu) | ((r[k] >> 16) & 0xf0f0f0f0u); // values 1, 3
                 uint32_t w[4];
-                e2m1x8_to_f16x2x4(ev | (od << 16), w);                                  // 0, 2, 1, 3
+                e2m1x8_to_f16x2x4(prmt(ev, od, 0x5410u), w);                                    // 0, 2, 1, 3
                 v[k][0] = hmul2_u32(w[0], s2);
                 v[k][2] = hmul2_u32(w[1], s2);
                 v[k][1] = hmul2_u32(w[2], s2);
@@ -489,10 +491,11 @@ __global__ void __launch_bounds__(C::NT) block_decode_kernel(const BlockDecodeAr
 template <int D, int FMT>
 cudaError_t launch(const BlockDecodeArgs& a, cudaStream_t s) {
   using C = Cfg<D, FMT>;
-  // Few lists: each is split over a cluster until the SMs have a CTA each, as long as a CTA keeps two pages.
+  // Few lists: each is split over a cluster until every SM holds the CTAs it has room for, as long as a CTA keeps
+  // two pages.
   const int units = a.B * a.Hk;
   int cs = 1;
-  while (cs < 8 && units * cs * 2 <= 148 && a.budget >= 4 * cs) cs *= 2;
+  while (cs < 8 && units * cs * 2 <= 148 * C::RES && a.budget >= 4 * cs) cs *= 2;
   const int cap = (a.budget + cs - 1) / cs;
   const int smem = C::smem(cap);
   auto k = block_decode_kernel<C>;
