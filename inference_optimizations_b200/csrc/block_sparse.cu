@@ -29,10 +29,11 @@ __device__ __forceinline__ int code8(float v, float inv) {
 
 // ------------------------------------------------------------------------------------------ head vectors
 // A warp holds one head vector of D values: lane l owns D / 64 consecutive values of each half, so both members of
-// every rotated pair (i, i + D / 2) are in one thread.
+// every rotated pair (i, i + D / 2) are in one thread.  Values go in pairs: one instruction handles two fp32.
 template <int D>
 struct Lane {
-  static constexpr int H2 = D / 64, E = D / 32;
+  static constexpr int H2 = D / 64;     // values of one half
+  static constexpr int P = H2 / 2;      // pairs of one half
 };
 
 template <int BYTES>
@@ -40,320 +41,446 @@ struct Raw;
 template <> struct Raw<1> { using T = uint8_t; };
 template <> struct Raw<2> { using T = uint16_t; };
 template <> struct Raw<4> { using T = uint32_t; };
-template <> struct Raw<8> { using T = uint2; };
-template <> struct Raw<16> { using T = uint4; };
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\t"
+      "fma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;\n\t}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 bf2(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t to_bf2(float2 v) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A lane's share of a bf16 head vector as it lies in memory: pairs 0 .. P - 1 of the first half, then the second's.
 template <int D>
-__device__ __forceinline__ void load_bf16(const __nv_bfloat16* src, int lane, float (&x)[D / 32]) {
-  constexpr int H2 = Lane<D>::H2;
-  using T = typename Raw<2 * H2>::T;
-#pragma unroll
-  for (int hh = 0; hh < 2; ++hh) {
-    const T raw = *reinterpret_cast<const T*>(src + hh * (D / 2) + lane * H2);
-    const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&raw);
-#pragma unroll
-    for (int j = 0; j < H2; ++j) x[hh * H2 + j] = __bfloat162float(e[j]);
+struct Head {
+  uint32_t w[2 * Lane<D>::P];
+};
+template <int P>
+__device__ __forceinline__ void load_words(const void* src, uint32_t* w) {
+  if constexpr (P == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(src);
+  } else if constexpr (P == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(src);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(src);
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
   }
+}
+template <int P>
+__device__ __forceinline__ void store_words(void* dst, const uint32_t* w) {
+  if constexpr (P == 1) *reinterpret_cast<uint32_t*>(dst) = w[0];
+  else if constexpr (P == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <int D>
-__device__ __forceinline__ void store_bf16(__nv_bfloat16* dst, int lane, const float (&x)[D / 32]) {
-  constexpr int H2 = Lane<D>::H2;
-  using T = typename Raw<2 * H2>::T;
+__device__ __forceinline__ Head<D> fetch(const __nv_bfloat16* src, int lane) {
+  Head<D> r;
 #pragma unroll
-  for (int hh = 0; hh < 2; ++hh) {
-    T raw;
-    __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(&raw);
+  for (int hh = 0; hh < 2; ++hh) load_words<Lane<D>::P>(src + hh * (D / 2) + lane * Lane<D>::H2, &r.w[hh * Lane<D>::P]);
+  return r;
+}
+template <int D>
+__device__ __forceinline__ void store_head(__nv_bfloat16* dst, int lane, const Head<D>& r) {
 #pragma unroll
-    for (int j = 0; j < H2; ++j) e[j] = __float2bfloat16(x[hh * H2 + j]);
-    *reinterpret_cast<T*>(dst + hh * (D / 2) + lane * H2) = raw;
+  for (int hh = 0; hh < 2; ++hh) store_words<Lane<D>::P>(dst + hh * (D / 2) + lane * Lane<D>::H2, &r.w[hh * Lane<D>::P]);
+}
+
+// What a stored row holds, as 16-bit pairs in units of the pool's scale: bf16, or f16 for E4M3 values and for E2M1
+// codes times their block's scale (both exact).
+template <int FMT>
+__device__ __forceinline__ float2 pair_value(uint32_t w) {
+  if constexpr (FMT == kKvBf16) return bf2(w);
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// H2 E2M1 codes of one word (lowest nibble first) -> pairs of code * block scale in f16.  Twice the magnitudes
+// {0, .5, 1, 1.5, 2, 3, 4, 6} are the bytes of a two-word table that a byte permute indexes; as f16 integers (an
+// exponent glued to the byte, 1024 taken off) they are exact, and so are the products.
+template <int H2>
+__device__ __forceinline__ void widen_e2m1(uint32_t word, float sf, uint32_t* pairs) {
+  const __half2 half_sf = __float2half2_rn(0.5f * sf);
+#pragma unroll
+  for (int j = 0; j < H2; j += 2) {
+    const uint32_t c = (word >> (4 * j)) & 0x77u;
+    uint32_t m = prmt(0x03020100u, 0x0C080604u, c) & 0xffffu;                 // two magnitude bytes
+    m = prmt(m, 0x64646464u, 0x4140u);                                        // 1024 + magnitude, f16 pair
+    __half2 v = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&m), __float2half2_rn(1024.f)), half_sf);
+    const uint32_t sg = word >> (4 * j);
+    pairs[j / 2] = *reinterpret_cast<uint32_t*>(&v) | ((sg & 8u) << 12) | ((sg & 0x80u) << 24);
   }
 }
 
-// N E2M1 codes of one word (lowest nibble first) -> code * block scale * global scale.  Twice the magnitudes
-// {0, .5, 1, 1.5, 2, 3, 4, 6} are the bytes of a two-word table that a byte permute indexes.
-template <int N>
-__device__ __forceinline__ void widen_e2m1(uint32_t word, float sf, float scale, float* x) {
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const uint32_t c = word >> (4 * j);
-    const float m = 0.5f * static_cast<float>(prmt(0x03020100u, 0x0C080604u, c & 7u) & 0xffu);
-    x[j] = ((c & 8u) ? -m : m) * sf * scale;
-  }
-}
-
-// One row of a pool part (K or V of a page and head): stores x (one rounding, from fp32) and replaces it by the
-// values the stored row stands for.
+// One row of a pool part (K or V of a page and head): stores x (one rounding, from fp32; `inv` is 1 / the pool's
+// scale) and returns what the row holds.  A reciprocal product instead of a division moves a value by 2^-24 of
+// itself, far below the formats' steps.
 template <int D, int FMT>
-__device__ __forceinline__ void store_row(uint8_t* part, int off, int lane, float scale, float (&x)[D / 32]) {
-  constexpr int H2 = Lane<D>::H2;
+__device__ __forceinline__ Head<D> store_row(uint8_t* part, int off, int lane, float inv,
+                                             const float2 (&x)[2 * Lane<D>::P]) {
+  constexpr int H2 = Lane<D>::H2, P = Lane<D>::P;
+  Head<D> out;
 #pragma unroll
   for (int hh = 0; hh < 2; ++hh) {
     const int e0 = hh * (D / 2) + lane * H2;
     if constexpr (FMT == kKvBf16) {
-      using T = typename Raw<2 * H2>::T;
-      T raw;
-      __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(&raw);
 #pragma unroll
-      for (int j = 0; j < H2; ++j) {
-        e[j] = __float2bfloat16(x[hh * H2 + j]);
-        x[hh * H2 + j] = __bfloat162float(e[j]);
-      }
-      *reinterpret_cast<T*>(part + off * 2 * D + kv_swizzle_byte(2 * e0, off, 2 * D)) = raw;
+      for (int j = 0; j < P; ++j) out.w[hh * P + j] = to_bf2(x[hh * P + j]);
+      store_words<P>(part + off * 2 * D + kv_swizzle_byte(2 * e0, off, 2 * D), &out.w[hh * P]);
     } else if constexpr (FMT == kKvFp8) {
-      using T = typename Raw<H2>::T;
-      T raw;
-      uint8_t* e = reinterpret_cast<uint8_t*>(&raw);
+      uint32_t word[P > 1 ? P / 2 : 1] = {};
 #pragma unroll
-      for (int j = 0; j < H2; ++j) {
-        e[j] = float_to_e4m3(x[hh * H2 + j] / scale);
-        x[hh * H2 + j] = e4m3_to_float(e[j]) * scale;
+      for (int j = 0; j < P; ++j) {
+        const uint32_t e = f32x2_to_e4m3x2(x[hh * P + j].x * inv, x[hh * P + j].y * inv);
+        out.w[hh * P + j] = e4m3x2_to_f16x2(static_cast<uint16_t>(e));
+        word[j / 2] |= e << (16 * (j & 1));
       }
-      *reinterpret_cast<T*>(part + off * D + kv_swizzle_byte(e0, off, D)) = raw;
+      uint8_t* dst = part + off * D + kv_swizzle_byte(e0, off, D);
+      if constexpr (P == 1) *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(word[0]);
+      else if constexpr (P == 2) *reinterpret_cast<uint32_t*>(dst) = word[0];
+      else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
     } else {
       constexpr int LPB = 16 / H2;       // lanes per 16-value block
       using T = typename Raw<(H2 / 2 > 0 ? H2 / 2 : 1)>::T;
+      float2 y[P];
       float amax = 0.f;
 #pragma unroll
-      for (int j = 0; j < H2; ++j) {
-        x[hh * H2 + j] /= scale;
-        amax = fmaxf(amax, fabsf(x[hh * H2 + j]));
+      for (int j = 0; j < P; ++j) {
+        y[j] = make_float2(x[hh * P + j].x * inv, x[hh * P + j].y * inv);
+        amax = fmaxf(amax, fmaxf(fabsf(y[j].x), fabsf(y[j].y)));
       }
 #pragma unroll
       for (int o = 1; o < LPB; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       const uint8_t s8 = nvfp4_block_scale(amax);
-      const float sf = e4m3_to_float(s8);
+      const float sf = e4m3_to_float(s8), inv_sf = 1.f / sf;
       if ((lane % LPB) == 0) part[kPage * (D / 2) + off * (D / 16) + e0 / 16] = s8;
       uint32_t word = 0;
 #pragma unroll
-      for (int j = 0; j < H2; ++j) word |= e2m1_code(x[hh * H2 + j] / sf) << (4 * j);
+      for (int j = 0; j < P; ++j)
+        word |= (e2m1_code(y[j].x * inv_sf) | (e2m1_code(y[j].y * inv_sf) << 4)) << (8 * j);
       *reinterpret_cast<T*>(part + off * (D / 2) + kv_swizzle_byte(e0 / 2, off, D / 2)) = static_cast<T>(word);
-      widen_e2m1<H2>(word, sf, scale, &x[hh * H2]);
+      widen_e2m1<H2>(word, sf, &out.w[hh * P]);
     }
   }
+  return out;
 }
 
 template <int D, int FMT>
-__device__ __forceinline__ void load_row(const uint8_t* part, int off, int lane, float scale, float (&x)[D / 32]) {
-  constexpr int H2 = Lane<D>::H2;
+__device__ __forceinline__ Head<D> load_row(const uint8_t* part, int off, int lane) {
+  constexpr int H2 = Lane<D>::H2, P = Lane<D>::P;
+  Head<D> out;
 #pragma unroll
   for (int hh = 0; hh < 2; ++hh) {
     const int e0 = hh * (D / 2) + lane * H2;
     if constexpr (FMT == kKvBf16) {
-      using T = typename Raw<2 * H2>::T;
-      const T raw = *reinterpret_cast<const T*>(part + off * 2 * D + kv_swizzle_byte(2 * e0, off, 2 * D));
-      const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&raw);
-#pragma unroll
-      for (int j = 0; j < H2; ++j) x[hh * H2 + j] = __bfloat162float(e[j]);
+      load_words<P>(part + off * 2 * D + kv_swizzle_byte(2 * e0, off, 2 * D), &out.w[hh * P]);
     } else if constexpr (FMT == kKvFp8) {
-      using T = typename Raw<H2>::T;
-      const T raw = *reinterpret_cast<const T*>(part + off * D + kv_swizzle_byte(e0, off, D));
-      const uint8_t* e = reinterpret_cast<const uint8_t*>(&raw);
+      const uint8_t* src = part + off * D + kv_swizzle_byte(e0, off, D);
+      uint2 word = make_uint2(0, 0);
+      if constexpr (P == 1) word.x = *reinterpret_cast<const uint16_t*>(src);
+      else if constexpr (P == 2) word.x = *reinterpret_cast<const uint32_t*>(src);
+      else word = *reinterpret_cast<const uint2*>(src);
 #pragma unroll
-      for (int j = 0; j < H2; ++j) x[hh * H2 + j] = e4m3_to_float(e[j]) * scale;
+      for (int j = 0; j < P; ++j)
+        out.w[hh * P + j] = e4m3x2_to_f16x2(static_cast<uint16_t>((j < 2 ? word.x : word.y) >> (16 * (j & 1))));
     } else {
       using T = typename Raw<(H2 / 2 > 0 ? H2 / 2 : 1)>::T;
       const float sf = e4m3_to_float(part[kPage * (D / 2) + off * (D / 16) + e0 / 16]);
-      const T raw = *reinterpret_cast<const T*>(part + off * (D / 2) + kv_swizzle_byte(e0 / 2, off, D / 2));
-      widen_e2m1<H2>(raw, sf, scale, &x[hh * H2]);
+      const uint32_t word = *reinterpret_cast<const T*>(part + off * (D / 2) + kv_swizzle_byte(e0 / 2, off, D / 2));
+      widen_e2m1<H2>(word, sf, &out.w[hh * P]);
     }
   }
+  return out;
 }
 
-// Norm (per head, optional) and rotation in fp32; nothing is rounded in between.
+// Cosines and sines of one position, this lane's pairs.
 template <int D>
-__device__ __forceinline__ void norm_rope(float (&x)[D / 32], const __nv_bfloat16* w, float eps, bool plus_one,
-                                          const float* cs, int lane) {
-  constexpr int H2 = Lane<D>::H2, E = Lane<D>::E;
-  if (w) {
-    float ss = 0.f;
+struct Angles {
+  float2 c[Lane<D>::P], s[Lane<D>::P], ns[Lane<D>::P];
+  __device__ __forceinline__ void load(const float* cs, int lane) {
+    constexpr int H2 = Lane<D>::H2;
+    const float* cl = cs + lane * H2;
+    if constexpr (H2 == 2) {
+      c[0] = *reinterpret_cast<const float2*>(cl);
+      s[0] = *reinterpret_cast<const float2*>(cl + D / 2);
+    } else {
 #pragma unroll
-    for (int j = 0; j < E; ++j) ss += x[j] * x[j];
-    const float inv = rsqrtf(warp_sum(ss) / D + eps);
-    float g[E];
-    load_bf16<D>(w, lane, g);
+      for (int j = 0; j < H2; j += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(cl + j), v = *reinterpret_cast<const float4*>(cl + D / 2 + j);
+        c[j / 2] = make_float2(u.x, u.y);
+        c[j / 2 + 1] = make_float2(u.z, u.w);
+        s[j / 2] = make_float2(v.x, v.y);
+        s[j / 2 + 1] = make_float2(v.z, v.w);
+      }
+    }
 #pragma unroll
-    for (int j = 0; j < E; ++j) x[j] = x[j] * inv * (plus_one ? 1.f + g[j] : g[j]);
+    for (int j = 0; j < H2 / 2; ++j) ns[j] = make_float2(-s[j].x, -s[j].y);
+  }
+};
+
+// Norm (per head, optional) and rotation in fp32; nothing is rounded in between.  `gain` is the lane's share of the
+// norm's weight.
+template <int D>
+__device__ __forceinline__ void norm_rope(const Head<D>& raw, float2 (&x)[2 * Lane<D>::P],
+                                          const float2 (&gain)[2 * Lane<D>::P], bool norm, float eps,
+                                          const Angles<D>& an) {
+  constexpr int P = Lane<D>::P;
+#pragma unroll
+  for (int j = 0; j < 2 * P; ++j) x[j] = bf2(raw.w[j]);
+  if (norm) {
+    float2 ss = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 2 * P; ++j) ss = fma2(x[j], x[j], ss);
+    const float inv = rsqrtf(warp_sum(ss.x + ss.y) / D + eps);
+#pragma unroll
+    for (int j = 0; j < 2 * P; ++j) x[j] = mul2(mul2(x[j], make_float2(inv, inv)), gain[j]);
   }
 #pragma unroll
-  for (int j = 0; j < H2; ++j) {
-    const float c = cs[lane * H2 + j], s = cs[D / 2 + lane * H2 + j];
-    const float a = x[j], b = x[H2 + j];
-    x[j] = a * c - b * s;
-    x[H2 + j] = b * c + a * s;
+  for (int j = 0; j < P; ++j) {
+    const float2 a = x[j], b = x[P + j];
+    x[j] = fma2(b, an.ns[j], mul2(a, an.c[j]));
+    x[P + j] = fma2(a, an.s[j], mul2(b, an.c[j]));
+  }
+}
+template <int D>
+__device__ __forceinline__ void load_gain(const void* w, bool plus_one, int lane, float2 (&gain)[2 * Lane<D>::P]) {
+  const Head<D> r = fetch<D>(reinterpret_cast<const __nv_bfloat16*>(w), lane);
+#pragma unroll
+  for (int j = 0; j < 2 * Lane<D>::P; ++j) {
+    gain[j] = bf2(r.w[j]);
+    if (plus_one) gain[j] = make_float2(1.f + gain[j].x, 1.f + gain[j].y);
   }
 }
 
-// Running bound of the rows seen by this lane, and the CTA-wide end of it: codes and scale of one page and head.
-template <int D>
+// Running bound of the rows seen by this lane, in the rows' 16-bit pairs (nothing is rounded; the pool's scale is
+// positive).  NaN stays NaN.
+template <int D, int FMT>
 struct Bound {
-  float lo[D / 32], hi[D / 32];
-  bool bad;                             // a key was not finite
+  uint32_t lo[2 * Lane<D>::P], hi[2 * Lane<D>::P];
+  static constexpr uint32_t kInf = FMT == kKvBf16 ? 0x7f807f80u : 0x7c007c00u;
+  static __device__ __forceinline__ uint32_t low(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (FMT == kKvBf16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t high(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (FMT == kKvBf16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
   __device__ __forceinline__ void reset() {
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) { lo[j] = INFINITY; hi[j] = -INFINITY; }
-    bad = false;
+    for (int j = 0; j < 2 * Lane<D>::P; ++j) { lo[j] = kInf; hi[j] = kInf | 0x80008000u; }
   }
-  __device__ __forceinline__ void add(const float (&x)[D / 32]) {
+  __device__ __forceinline__ void add(const Head<D>& r) {
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      lo[j] = fminf(lo[j], x[j]);
-      hi[j] = fmaxf(hi[j], x[j]);
-      bad |= !(fabsf(x[j]) < INFINITY);
-    }
+    for (int j = 0; j < 2 * Lane<D>::P; ++j) { lo[j] = low(lo[j], r.w[j]); hi[j] = high(hi[j], r.w[j]); }
   }
 };
 
 constexpr int kWarps = 4;
 
-template <int D>
-__device__ void finish_bound(const Bound<D>& bd, int8_t* codes, __nv_bfloat16* scale, float* smem) {
-  constexpr int H2 = Lane<D>::H2;
+// End of a page's bound: the warps' shares are joined and the codes and the scale of one page and head written.
+template <int D, int FMT>
+__device__ void finish_bound(const Bound<D, FMT>& bd, float unit, int8_t* codes, __nv_bfloat16* scale,
+                             uint32_t (&sb)[2][kWarps][D / 2]) {
+  constexpr int P = Lane<D>::P, NT = kWarps * 32;
   const int lane = lane_id(), warp = warp_id();
-  float* slo = smem;                    // [kWarps][D]
-  float* shi = smem + kWarps * D;
   __shared__ float smax[kWarps];
-  __shared__ int sbad;
-  if (threadIdx.x == 0) sbad = 0;
-  __syncthreads();
 #pragma unroll
   for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-    for (int j = 0; j < H2; ++j) {
-      slo[warp * D + hh * (D / 2) + lane * H2 + j] = bd.lo[hh * H2 + j];
-      shi[warp * D + hh * (D / 2) + lane * H2 + j] = bd.hi[hh * H2 + j];
+    for (int j = 0; j < P; ++j) {
+      const int d = hh * (D / 4) + lane * P + j;
+      sb[0][warp][d] = bd.lo[hh * P + j];
+      sb[1][warp][d] = bd.hi[hh * P + j];
     }
-  if (bd.bad) sbad = 1;
   __syncthreads();
-  constexpr int PER = D / (kWarps * 32);
-  float c[PER], w[PER], amax = 0.f;
+  constexpr int PER = D / 2 >= NT ? D / 2 / NT : 1;       // pairs of a thread (threads past D / 2 idle)
+  const int d0 = threadIdx.x * PER;
+  float c[2 * PER], w[2 * PER], amax = 0.f;
+  bool bad = false;
+  if (d0 < D / 2) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int d = threadIdx.x * PER + i;
-    float lo = slo[d], hi = shi[d];
+    for (int i = 0; i < PER; ++i) {
+      uint32_t l = sb[0][0][d0 + i], h = sb[1][0][d0 + i];
 #pragma unroll
-    for (int k = 1; k < kWarps; ++k) { lo = fminf(lo, slo[k * D + d]); hi = fmaxf(hi, shi[k * D + d]); }
-    c[i] = (lo + hi) * 0.5f;
-    w[i] = (hi - lo) * 0.5f;
-    amax = fmaxf(amax, fmaxf(fabsf(c[i]), w[i]));
+      for (int k = 1; k < kWarps; ++k) {
+        l = Bound<D, FMT>::low(l, sb[0][k][d0 + i]);
+        h = Bound<D, FMT>::high(h, sb[1][k][d0 + i]);
+      }
+      const float2 lv = pair_value<FMT>(l), hv = pair_value<FMT>(h);
+      const float lo2[2] = {lv.x * unit, lv.y * unit}, hi2[2] = {hv.x * unit, hv.y * unit};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        c[2 * i + k] = (lo2[k] + hi2[k]) * 0.5f;
+        w[2 * i + k] = (hi2[k] - lo2[k]) * 0.5f;
+        bad |= !(fabsf(lo2[k]) < INFINITY && fabsf(hi2[k]) < INFINITY);
+        amax = fmaxf(amax, fmaxf(fabsf(c[2 * i + k]), w[2 * i + k]));
+      }
+    }
   }
+  if (bad) amax = INFINITY;                       // as an overflow of lo + hi or hi - lo
   amax = warp_max(amax);
   if (lane == 0) smax[warp] = amax;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kWarps; ++k) amax = fmaxf(amax, smax[k]);
-  const bool bad = sbad != 0 || !(amax < INFINITY);     // (lo + hi or hi - lo may overflow)
+  bad = !(amax < INFINITY);
   const int e = code_exp(amax);
   const float inv = pow2(-e);
-  using T = typename Raw<PER>::T;
-  T rc, rw;
+  using T = typename Raw<2 * PER>::T;
+  if (d0 < D / 2) {
+    uint32_t rc = 0, rw = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    reinterpret_cast<int8_t*>(&rc)[i] = static_cast<int8_t>(bad ? 0 : code8(c[i], inv));
-    reinterpret_cast<int8_t*>(&rw)[i] = static_cast<int8_t>(bad ? 0 : code8(w[i], inv));
+    for (int i = 0; i < 2 * PER; ++i) {
+      rc |= (bad ? 0u : static_cast<uint32_t>(code8(c[i], inv)) & 0xffu) << (8 * i);
+      rw |= (bad ? 0u : static_cast<uint32_t>(code8(w[i], inv)) & 0xffu) << (8 * i);
+    }
+    reinterpret_cast<T*>(codes)[threadIdx.x] = static_cast<T>(rc);
+    reinterpret_cast<T*>(codes + D)[threadIdx.x] = static_cast<T>(rw);
   }
-  reinterpret_cast<T*>(codes)[threadIdx.x] = rc;
-  reinterpret_cast<T*>(codes + D)[threadIdx.x] = rw;
   if (threadIdx.x == 0) *scale = __float2bfloat16(bad ? INFINITY : pow2(e));
-  __syncthreads();                      // smem is used again by the next run
+  __syncthreads();                                // shared memory is used again by the next run
 }
 
 // ------------------------------------------------------------------------------------------ append
-// Grid: x = slabs of `slab` rows; y < Hk: the K vectors of kv head y, else four of the Hq + Hk q and v vectors.
-// A K CTA owns the page runs that start in its slab (consecutive rows at consecutive slots of one page): its warps
-// share the run's rows, and when the run ends at the page's last row the CTA also reads the rows written by earlier
-// calls and writes the page's bound, so the bound costs no launch and no second pass over the new keys.
+// Grid: x = slabs of `slab` rows; y < Hk: the K vectors of kv head y, else `heads` of the Hq + Hk q and v vectors.
+// q and v: a warp takes a row and walks through the heads, the position's angles in registers and the next two heads'
+// values on their way.  K: a CTA owns the page runs that start in its slab (consecutive rows at consecutive slots of
+// one page): its warps share the run's rows, and when the run ends at the page's last row the CTA also reads the rows
+// written by earlier calls and writes the page's bound, so the bound costs no launch and no second pass over the new
+// keys.
 __device__ __forceinline__ int row_slot(const BlockAppendArgs& a, int t) {
   const int s = a.slot[t], p = a.pos[t];
   return (s < 0 || s >= a.slots || p < 0 || p >= a.max_pos) ? -1 : s;
 }
 
 template <int D, int FMT>
-__global__ void __launch_bounds__(kWarps * 32) block_append_kernel(const BlockAppendArgs a) {
-  __shared__ float red[2 * kWarps * D];
+__global__ void __launch_bounds__(kWarps * 32, D == 512 ? 5 : 6) block_append_kernel(const BlockAppendArgs a) {
+  __shared__ uint32_t red[2][kWarps][D / 2];
   const int warp = warp_id(), lane = lane_id();
   const int t0 = blockIdx.x * a.slab, t1 = min(a.T, t0 + a.slab);
   const __nv_bfloat16* qkv = reinterpret_cast<const __nv_bfloat16*>(a.qkv);
-  const int part = gqa_block_bytes(FMT, D, kPage) / 2;
-  float x[D / 32];
+  constexpr int part = FMT == kKvBf16 ? kPage * 2 * D : FMT == kKvFp8 ? kPage * D : kPage * (D / 2 + D / 16);
+  float2 x[2 * Lane<D>::P], gain[2 * Lane<D>::P];
+  Angles<D> an;
   if (static_cast<int>(blockIdx.y) >= a.Hk) {
-    const int v = (blockIdx.y - a.Hk) * kWarps + warp;
-    if (v >= a.Hq + a.Hk) return;
-    const bool is_q = v < a.Hq;
-    for (int t = t0; t < t1; ++t) {
-      const int src = is_q ? v : v + a.Hk;
-      load_bf16<D>(qkv + static_cast<size_t>(t) * a.qkv_stride + static_cast<size_t>(src) * D, lane, x);
-      if (is_q) {
-        const int p = a.pos[t];
-        __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.q_out) + (static_cast<size_t>(t) * a.Hq + v) * D;
-        if (p >= 0 && p < a.max_pos) {
-          norm_rope<D>(x, reinterpret_cast<const __nv_bfloat16*>(a.q_norm), a.eps, a.plus_one,
-                       a.cos_sin + static_cast<size_t>(p) * D, lane);
-        } else {
+    // a warp per row where there are rows for it, else a warp per head
+    const int first = (blockIdx.y - a.Hk) * a.heads;
+    const int vend = min(first + a.heads, a.Hq + a.Hk);
+    const int v0 = first + (a.slab == 1 ? warp : 0), vstep = a.slab == 1 ? kWarps : 1;
+    if (v0 >= vend) return;
+    if (a.q_norm && v0 < a.Hq) load_gain<D>(a.q_norm, a.plus_one, lane, gain);
+    const float inv = FMT == kKvBf16 ? 1.f : 1.f / a.v_scale;
+    for (int t = t0 + (a.slab == 1 ? 0 : warp); t < t1; t += (a.slab == 1 ? 1 : kWarps)) {
+      const __nv_bfloat16* src = qkv + static_cast<size_t>(t) * a.qkv_stride;
+      auto head = [&](int v) { return fetch<D>(src + static_cast<size_t>(v < a.Hq ? v : v + a.Hk) * D, lane); };
+      Head<D> next = head(v0), next2{};
+      if (v0 + vstep < vend) next2 = head(v0 + vstep);
+      const int p = a.pos[t], s = row_slot(a, t);
+      const bool ok = p >= 0 && p < a.max_pos;
+      if (ok && v0 < a.Hq) an.load(a.cos_sin + static_cast<size_t>(p) * D, lane);
+      __nv_bfloat16* qrow = reinterpret_cast<__nv_bfloat16*>(a.q_out) + static_cast<size_t>(t) * a.Hq * D;
+      uint8_t* vrow = a.pool + static_cast<size_t>(s < 0 ? 0 : s / kPage) * a.Hk * (2 * part) + part;
+      for (int v = v0; v < vend; v += vstep) {
+        const Head<D> raw = next;
+        const int vn = v + 2 * vstep;
+        next = next2;
+        if (vn < vend) next2 = head(vn);
+        if (v < a.Hq) {
+          Head<D> o{};
+          if (ok) {
+            norm_rope<D>(raw, x, gain, a.q_norm != nullptr, a.eps, an);
 #pragma unroll
-          for (int j = 0; j < D / 32; ++j) x[j] = 0.f;
+            for (int j = 0; j < 2 * Lane<D>::P; ++j) o.w[j] = to_bf2(x[j]);
+          }
+          store_head<D>(qrow + static_cast<size_t>(v) * D, lane, o);
+        } else if (s >= 0) {
+#pragma unroll
+          for (int j = 0; j < 2 * Lane<D>::P; ++j) x[j] = bf2(raw.w[j]);
+          store_row<D, FMT>(vrow + static_cast<size_t>(v - a.Hq) * (2 * part), s % kPage, lane, inv, x);
         }
-        store_bf16<D>(dst, lane, x);
-      } else {
-        const int s = row_slot(a, t);
-        if (s < 0) continue;
-        uint8_t* base = a.pool + (static_cast<size_t>(s / kPage) * a.Hk + (v - a.Hq)) * (2 * part) + part;
-        store_row<D, FMT>(base, s % kPage, lane, a.v_scale, x);
       }
     }
     return;
   }
   const int h = blockIdx.y;
+  const float unit = FMT == kKvBf16 ? 1.f : a.k_scale, inv = 1.f / unit;
+  if (a.k_norm) load_gain<D>(a.k_norm, a.plus_one, lane, gain);
   for (int t = t0; t < t1; ++t) {
     const int s = row_slot(a, t);
     if (s < 0) continue;
-    if (t > 0 && (s % kPage) != 0 && row_slot(a, t - 1) == s - 1) continue;      // inside a run that began before
-    int n = 1;                            // rows of the run (at most a page)
-    while (s % kPage + n < kPage && t + n < a.T && row_slot(a, t + n) == s + n) ++n;
     const int page = s / kPage, off = s % kPage;
+    if (t > 0 && off != 0 && row_slot(a, t - 1) == s - 1) continue;              // inside a run that began before
+    // rows of the run (at most to the page's end): every lane looks at two
+    bool in0 = off + lane < kPage && t + lane < a.T, in1 = off + lane + 32 < kPage && t + lane + 32 < a.T;
+    in0 = in0 && row_slot(a, t + lane) == s + lane;
+    in1 = in1 && row_slot(a, t + lane + 32) == s + lane + 32;
+    const unsigned long long in = __ballot_sync(0xffffffffu, in0) |
+                                  static_cast<unsigned long long>(__ballot_sync(0xffffffffu, in1)) << 32;
+    const int n = ~in == 0ull ? kPage : __ffsll(~in) - 1;
     const bool last = off + n == kPage;
     uint8_t* base = a.pool + (static_cast<size_t>(page) * a.Hk + h) * (2 * part);
-    Bound<D> bd;
+    Bound<D, FMT> bd;
     bd.reset();
+    const __nv_bfloat16* src = qkv + static_cast<size_t>(t) * a.qkv_stride + static_cast<size_t>(a.Hq + h) * D;
+    Head<D> next;
+    if (warp < n) next = fetch<D>(src + warp * a.qkv_stride, lane);
     for (int i = warp; i < n; i += kWarps) {
-      load_bf16<D>(qkv + static_cast<size_t>(t + i) * a.qkv_stride + static_cast<size_t>(a.Hq + h) * D, lane, x);
-      norm_rope<D>(x, reinterpret_cast<const __nv_bfloat16*>(a.k_norm), a.eps, a.plus_one,
-                   a.cos_sin + static_cast<size_t>(a.pos[t + i]) * D, lane);
-      store_row<D, FMT>(base, off + i, lane, a.k_scale, x);
-      bd.add(x);
+      an.load(a.cos_sin + static_cast<size_t>(a.pos[t + i]) * D, lane);
+      const Head<D> raw = next;
+      if (i + kWarps < n) next = fetch<D>(src + (i + kWarps) * a.qkv_stride, lane);
+      norm_rope<D>(raw, x, gain, a.k_norm != nullptr, a.eps, an);
+      bd.add(store_row<D, FMT>(base, off + i, lane, inv, x));
     }
     if (!last) continue;
-    for (int i = warp; i < off; i += kWarps) {
-      load_row<D, FMT>(base, i, lane, a.k_scale, x);
-      bd.add(x);
-    }
+#pragma unroll 4
+    for (int i = warp; i < off; i += kWarps) bd.add(load_row<D, FMT>(base, i, lane));
     const size_t ph = static_cast<size_t>(page) * a.Hk + h;
-    finish_bound<D>(bd, a.codes + ph * 2 * D, reinterpret_cast<__nv_bfloat16*>(a.scale) + ph, red);
+    finish_bound<D, FMT>(bd, unit, a.codes + ph * 2 * D, reinterpret_cast<__nv_bfloat16*>(a.scale) + ph, red);
   }
 }
 
 // Bounds of whole pages from their stored keys: one CTA per (page of the list, kv head).
 template <int D, int FMT>
 __global__ void __launch_bounds__(kWarps * 32) block_summarize_kernel(const BlockAppendArgs a, const int* pages) {
-  __shared__ float red[2 * kWarps * D];
+  __shared__ uint32_t red[2][kWarps][D / 2];
   const int page = pages[blockIdx.x], h = blockIdx.y;
   if (page < 0 || page >= a.slots / kPage) return;
-  const int part = gqa_block_bytes(FMT, D, kPage) / 2;
+  constexpr int part = FMT == kKvBf16 ? kPage * 2 * D : FMT == kKvFp8 ? kPage * D : kPage * (D / 2 + D / 16);
   const uint8_t* base = a.pool + (static_cast<size_t>(page) * a.Hk + h) * (2 * part);
-  Bound<D> bd;
+  Bound<D, FMT> bd;
   bd.reset();
-  float x[D / 32];
 #pragma unroll 4
-  for (int i = warp_id(); i < kPage; i += kWarps) {
-    load_row<D, FMT>(base, i, lane_id(), a.k_scale, x);
-    bd.add(x);
-  }
+  for (int i = warp_id(); i < kPage; i += kWarps) bd.add(load_row<D, FMT>(base, i, lane_id()));
   const size_t ph = static_cast<size_t>(page) * a.Hk + h;
-  finish_bound<D>(bd, a.codes + ph * 2 * D, reinterpret_cast<__nv_bfloat16*>(a.scale) + ph, red);
+  finish_bound<D, FMT>(bd, FMT == kKvBf16 ? 1.f : a.k_scale, a.codes + ph * 2 * D,
+                       reinterpret_cast<__nv_bfloat16*>(a.scale) + ph, red);
 }
 
 // ------------------------------------------------------------------------------------------ select
-constexpr int kSelThreads = 256;
-
 // m16n8k32, 8-bit codes, 32-bit sums.
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
@@ -369,118 +496,194 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// One CTA per (group, kv head).  Scores: the 16 query rows' codes [q8 | |q8|] are the A operand (shared memory, rows
-// padded by 64 bytes: conflict-free 16-byte reads), 8 pages' records of 2 D codes the B operand, read once from
-// global memory, 16 bytes a thread; the products' k order is permuted alike on both sides so that a thread's 16 bytes are
-// two instructions' fragments.  Then a radix selection over the scores' order keys in shared memory.
-template <int D>
-__global__ void __launch_bounds__(kSelThreads) block_select_kernel(const BlockSelectArgs a) {
+// One cluster of C CTAs per (group, kv head); the CTAs share the candidate pages, the first one selects.
+// Scores: the 16 query rows' codes [q8 | |q8|] are the A operand (shared memory, rows padded by 64 bytes:
+// conflict-free 16-byte reads), 8 pages' records of 2 D codes the B operand, read once from global memory, 16 bytes a
+// thread and 16 of them in flight; the products' k order is permuted alike on both sides so that a thread's 16 bytes
+// are two instructions' fragments.  Every CTA stores its scores' order keys in the first CTA's shared memory.
+// Selection: radix, eight bits at a time from the highest bit in which the keys differ (scores share their leading
+// bits, which would put every key in one bin), ending as soon as a digit's bin is taken whole.
+template <int D, bool R8, int NT, int PP, int RES>
+__global__ void __launch_bounds__(NT, RES) block_select_kernel(const BlockSelectArgs a, const int csize) {
   constexpr int RS = 2 * D + 64;        // bytes between query rows
+  constexpr int U = 2 * D / 64;         // 64-byte pieces of a record
+  constexpr int NWARP = NT / 32;
   extern __shared__ __align__(16) uint8_t dyn[];
   int8_t* qs = reinterpret_cast<int8_t*>(dyn);                     // [16][RS]
-  uint32_t* keys = reinterpret_cast<uint32_t*>(dyn + 16 * RS);     // [N]
+  uint32_t* keys = reinterpret_cast<uint32_t*>(dyn + 16 * RS);     // [N] (first CTA of the cluster)
   __shared__ float rscale[16];
   __shared__ int hist[256];
-  __shared__ int wsum[kSelThreads / 32];
-  __shared__ int sdigit, sneed;
-  const int b = blockIdx.x, h = blockIdx.y;
+  __shared__ uint32_t wmin[NWARP], wmax[NWARP];
+  __shared__ int wsum[NWARP];
+  __shared__ int sdigit, sneed, scnt;
+  const int b = blockIdx.x / csize, rank = blockIdx.x % csize, h = blockIdx.y;
   const int tid = threadIdx.x, warp = warp_id(), lane = lane_id();
   const int row = a.req_idx ? a.req_idx[b] : b;
   const int G = a.Hq / a.Hk, R = a.n_q * G;
   int* out = a.blocks + (static_cast<size_t>(b) * a.Hk + h) * a.budget;
   const int len = (row < 0 || row >= a.rows) ? 0 : min(a.kv_len[b], a.pt_stride * kPage);
   const int npages = len > 0 ? (len + kPage - 1) / kPage : 0;
-  const int take = min(npages, a.budget);
-  if (tid == 0) a.count[static_cast<size_t>(b) * a.Hk + h] = take;
-  if (npages <= a.budget) {               // every page fits: nothing to rank
-    for (int j = tid; j < a.budget; j += kSelThreads) out[j] = j < npages ? j : -1;
-    return;
-  }
-  const int first_local = max(0, max(0, len - a.n_q) / kPage - (a.local - 1));
-  const int lo = a.sink, n = first_local - a.sink;                   // candidates [lo, lo + n)
-  const int want = a.budget - (npages - n);                          // how many of them are taken
-  // ---- query codes: one warp per row
-  for (int r = warp; r < 16; r += kSelThreads / 32) {
-    float amax = 0.f;
+  // ---- query codes, one warp per row (before the length is looked at: the loads overlap)
+#pragma unroll
+  for (int r = warp; r < (R8 ? 8 : 16); r += NWARP) {
     const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) +
                              static_cast<size_t>(b * a.n_q + r / G) * a.q_stride + (h * G + r % G) * D;
-    constexpr int V = D / 32;
-    float x[V];
+    constexpr int V = D / 32;             // consecutive values of a lane
+    float2 x[V / 2];
+    float amax = 0.f;
     bool bad = false;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      x[j] = r < R ? __bfloat162float(q[lane * V + j]) : 0.f;
-      amax = fmaxf(amax, fabsf(x[j]));
-      bad |= !(fabsf(x[j]) < INFINITY);
+    for (int j = 0; j < V / 2; j += (V < 8 ? V / 2 : 4)) {
+      uint32_t raw[V < 8 ? V / 2 : 4] = {};
+      if (r < R) load_words<(V < 8 ? V / 2 : 4)>(q + lane * V + 2 * j, raw);
+#pragma unroll
+      for (int k = 0; k < (V < 8 ? V / 2 : 4); ++k) {
+        x[j + k] = bf2(raw[k]);
+        amax = fmaxf(amax, fmaxf(fabsf(x[j + k].x), fabsf(x[j + k].y)));
+        bad |= !(fabsf(x[j + k].x) < INFINITY && fabsf(x[j + k].y) < INFINITY);
+      }
     }
     amax = warp_max(amax);
     bad = __any_sync(0xffffffffu, bad);
     const int e = code_exp(amax);
     const float inv = pow2(-e);
+    uint32_t wc[V / 4] = {}, wa[V / 4] = {};
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = bad ? 0 : code8(x[j], inv);
-      qs[r * RS + lane * V + j] = static_cast<int8_t>(c);
-      qs[r * RS + D + lane * V + j] = static_cast<int8_t>(abs(c));
+      const int c = bad ? 0 : code8((j & 1) ? x[j / 2].y : x[j / 2].x, inv);
+      wc[j / 4] |= (static_cast<uint32_t>(c) & 0xffu) << (8 * (j & 3));
+      wa[j / 4] |= static_cast<uint32_t>(abs(c)) << (8 * (j & 3));
     }
+    store_words<V / 4>(qs + r * RS + lane * V, wc);
+    store_words<V / 4>(qs + r * RS + D + lane * V, wa);
     if (lane == 0) rscale[r] = (r < R && !bad) ? pow2(e) : -1.f;
   }
-  __syncthreads();
-  // ---- scores: each warp 8 pages at a time
+  if (rank == 0 && tid == 0) a.count[static_cast<size_t>(b) * a.Hk + h] = min(npages, a.budget);
+  if (npages <= a.budget) {               // every page fits: nothing to rank (the whole cluster leaves here)
+    if (rank == 0)
+      for (int j = tid; j < a.budget; j += NT) out[j] = j < npages ? j : -1;
+    return;
+  }
+  const int first_local = max(0, max(0, len - a.n_q) / kPage - (a.local - 1));
+  const int lo = a.sink, n = first_local - a.sink;                   // candidates [lo, lo + n)
+  const int want = a.budget - (npages - n);                          // how many of them are taken
+  const int span = ((n + csize - 1) / csize + 7) & ~7;               // candidates of a CTA
+  const int c0 = min(n, rank * span), c1 = min(n, c0 + span);
   const int g = lane >> 2, j4 = lane & 3;
-  const float s0 = rscale[g], s1 = rscale[g + 8];
-  const int* pt = a.page_table + static_cast<size_t>(row) * a.pt_stride;
-  for (int p0 = warp * 8; p0 < n; p0 += kSelThreads / 32 * 8) {
-    const int mine = min(p0 + g, n - 1);
-    int phys = pt[lo + mine];
-    const bool ok = phys >= 0 && phys < a.pages;
-    if (!ok) phys = 0;
-    const size_t ph = static_cast<size_t>(phys) * a.Hk + h;
-    const uint4* rec = reinterpret_cast<const uint4*>(a.codes + ph * 2 * D) + j4;
-    int c[4] = {0, 0, 0, 0};
+  const int* pt = a.page_table + static_cast<size_t>(row) * a.pt_stride + lo;
+  int phys[PP];                           // pages of this thread's octets, loaded one step ahead
 #pragma unroll
-    for (int u = 0; u < 2 * D / 64; ++u) {
-      const uint4 bv = rec[4 * u];
-      const uint4 x = *reinterpret_cast<const uint4*>(qs + g * RS + 64 * u + 16 * j4);
-      const uint4 y = *reinterpret_cast<const uint4*>(qs + (g + 8) * RS + 64 * u + 16 * j4);
-      mma_s8(c, x.x, y.x, x.y, y.y, bv.x, bv.y);
-      mma_s8(c, x.z, y.z, x.w, y.w, bv.z, bv.w);
-    }
-    float m0 = -INFINITY, m1 = -INFINITY;           // pages p0 + 2 j4, p0 + 2 j4 + 1
-    if (s0 > 0.f) { m0 = static_cast<float>(c[0]) * s0; m1 = static_cast<float>(c[1]) * s0; }
-    if (s1 > 0.f) { m0 = fmaxf(m0, static_cast<float>(c[2]) * s1); m1 = fmaxf(m1, static_cast<float>(c[3]) * s1); }
+  for (int i = 0; i < PP; ++i) phys[i] = c1 > c0 ? pt[min(c0 + (warp * PP + i) * 8 + g, c1 - 1)] : 0;
+  if (csize > 1) cluster_sync_all();      // also: the first CTA runs, its shared memory may be written
+  else __syncthreads();
+  // ---- scores; the A operand stays in registers where it fits beside the records
+  constexpr bool AREG = PP == 1 && U * (R8 ? 4 : 8) <= 32;
+  uint4 ax[AREG ? U : 1], ay[AREG && !R8 ? U : 1];
+  if constexpr (AREG) {
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-      m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-    }
-    float sc = ok ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.scale)[ph]) : -1.f;
-    const float sc0 = __shfl_sync(0xffffffffu, sc, 8 * j4), sc1 = __shfl_sync(0xffffffffu, sc, 8 * j4 + 4);
-    if (g == 0) {
-      const int p = p0 + 2 * j4;
-      // a page whose keys are not finite ranks first, one outside the pool last
-      const float v0 = sc0 < 0.f ? -INFINITY : sc0 == INFINITY ? INFINITY : m0 * sc0;
-      const float v1 = sc1 < 0.f ? -INFINITY : sc1 == INFINITY ? INFINITY : m1 * sc1;
-      if (p < n) keys[p] = order_key(v0);
-      if (p + 1 < n) keys[p + 1] = order_key(v1);
+    for (int u = 0; u < U; ++u) {
+      ax[u] = *reinterpret_cast<const uint4*>(qs + g * RS + 64 * u + 16 * j4);
+      if constexpr (!R8) ay[u] = *reinterpret_cast<const uint4*>(qs + (g + 8) * RS + 64 * u + 16 * j4);
     }
   }
-  // ---- radix selection of the `want` largest keys, eight bits at a time
-  uint32_t prefix = 0, mask = 0;
-  int need = want;                                 // of the keys equal to the prefix so far
-  if (want == 0) prefix = 0xffffffffu;             // above every key: nothing is taken
-  for (int shift = want > 0 ? 24 : -8; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+  const float s0 = rscale[g], s1 = R8 ? -1.f : rscale[g + 8];
+  const uint32_t key_addr = csize > 1 ? mapa_shared(smem_u32(keys), 0) : smem_u32(keys);
+  for (int p0 = c0 + warp * PP * 8; p0 < c1; p0 += NWARP * PP * 8) {
+    uint4 bv[PP][U];
+    float sc[PP];
+#pragma unroll
+    for (int i = 0; i < PP; ++i) {
+      const bool ok = phys[i] >= 0 && phys[i] < a.pages;
+      const size_t ph = static_cast<size_t>(ok ? phys[i] : 0) * a.Hk + h;
+      const uint4* rec = reinterpret_cast<const uint4*>(a.codes + ph * 2 * D) + j4;
+#pragma unroll
+      for (int u = 0; u < U; ++u) bv[i][u] = rec[4 * u];
+      sc[i] = ok ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.scale)[ph]) : -1.f;
+    }
+    const int pn = p0 + NWARP * PP * 8;
+#pragma unroll
+    for (int i = 0; i < PP; ++i) phys[i] = pn < c1 ? pt[min(pn + i * 8 + g, c1 - 1)] : 0;
+    int c[PP][4];
+#pragma unroll
+    for (int i = 0; i < PP; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) c[i][k] = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint4 x, y = make_uint4(0, 0, 0, 0);
+      if constexpr (AREG) {
+        x = ax[u];
+        if constexpr (!R8) y = ay[u];
+      } else {
+        x = *reinterpret_cast<const uint4*>(qs + g * RS + 64 * u + 16 * j4);
+        if constexpr (!R8) y = *reinterpret_cast<const uint4*>(qs + (g + 8) * RS + 64 * u + 16 * j4);
+      }
+#pragma unroll
+      for (int i = 0; i < PP; ++i) {
+        mma_s8(c[i], x.x, y.x, x.y, y.y, bv[i][u].x, bv[i][u].y);
+        mma_s8(c[i], x.z, y.z, x.w, y.w, bv[i][u].z, bv[i][u].w);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PP; ++i) {
+      float m0 = -INFINITY, m1 = -INFINITY;           // pages 2 j4, 2 j4 + 1 of the octet
+      if (s0 > 0.f) { m0 = static_cast<float>(c[i][0]) * s0; m1 = static_cast<float>(c[i][1]) * s0; }
+      if (!R8 && s1 > 0.f) {
+        m0 = fmaxf(m0, static_cast<float>(c[i][2]) * s1);
+        m1 = fmaxf(m1, static_cast<float>(c[i][3]) * s1);
+      }
+      // largest of the rows: the first exchange leaves each lane one of its two pages, so that lanes 0 .. 7 end with
+      // page 2 (lane & 3) + (lane >> 2)
+      float m = (g & 1) ? m1 : m0;
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, (g & 1) ? m0 : m1, 4));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+      const int at = 2 * (lane & 3) + ((lane >> 2) & 1);
+      const float sp = __shfl_sync(0xffffffffu, sc[i], 4 * at);
+      const int p = p0 + 8 * i + at;
+      // a page whose keys are not finite ranks first, one outside the pool last
+      const float v = sp < 0.f ? -INFINITY : sp == INFINITY ? INFINITY : m * sp;
+      if (lane < 8 && p < c1)
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(key_addr + 4 * p), "r"(order_key(v)) : "memory");
+    }
+  }
+  if (csize > 1) {
+    cluster_sync_all();
+    if (rank != 0) return;                // nothing of this CTA is read any more
+  } else {
     __syncthreads();
-    for (int i = tid; i < n; i += kSelThreads) {
+  }
+  // ---- range of the keys: the digits start at the highest bit in which they differ
+  uint32_t kmin = 0xffffffffu, kmax = 0;
+  for (int i = tid; i < n; i += NT) {
+    const uint32_t k = keys[i];
+    kmin = min(kmin, k);
+    kmax = max(kmax, k);
+  }
+  kmin = __reduce_min_sync(0xffffffffu, kmin);
+  kmax = __reduce_max_sync(0xffffffffu, kmax);
+  if (lane == 0) { wmin[warp] = kmin; wmax[warp] = kmax; }
+  for (int i = tid; i < 256; i += NT) hist[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NWARP; ++w) { kmin = min(kmin, wmin[w]); kmax = max(kmax, wmax[w]); }
+  int top = 32 - __clz(kmin ^ kmax);               // bits that differ
+  uint32_t mask = top >= 32 ? 0u : 0xffffffffu << top;
+  uint32_t prefix = kmax & mask;
+  int need = want, cnt = n;                        // keys equal to the prefix: how many are taken, how many there are
+  if (want == 0) { mask = 0xffffffffu; prefix = 0xffffffffu; top = 0; }      // above every key
+  while (top > 0 && need < cnt) {
+    const int shift = max(0, top - 8);
+    const uint32_t digits = (1u << (top - shift)) - 1;
+    for (int i = tid; i < n; i += NT) {
       const uint32_t k = keys[i];
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1);
     }
     __syncthreads();
     if (warp == 0) {
-      int own = 0, cnt[8];                         // lane l: digits 255 - 8 l .. 248 - 8 l
+      int own = 0, c8[8];                          // lane l: digits 255 - 8 l .. 248 - 8 l
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { cnt[i] = hist[255 - 8 * lane - i]; own += cnt[i]; }
+      for (int i = 0; i < 8; ++i) { c8[i] = hist[255 - 8 * lane - i]; own += c8[i]; }
       int before = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -492,26 +695,30 @@ __global__ void __launch_bounds__(kSelThreads) block_select_kernel(const BlockSe
         int acc = before;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (acc < need && need <= acc + cnt[i]) { sdigit = 255 - 8 * lane - i; sneed = need - acc; }
-          acc += cnt[i];
+          if (acc < need && need <= acc + c8[i]) { sdigit = 255 - 8 * lane - i; sneed = need - acc; scnt = c8[i]; }
+          acc += c8[i];
         }
       }
     }
     __syncthreads();
+    for (int i = tid; i < 256; i += NT) hist[i] = 0;
     prefix |= static_cast<uint32_t>(sdigit) << shift;
-    mask |= 255u << shift;
+    mask |= digits << shift;
     need = sneed;
+    cnt = scnt;
+    top = shift;
+    __syncthreads();
   }
-  __syncthreads();
   // ---- compaction in page order: thread t owns a contiguous run of candidates
-  const int per = (n + kSelThreads - 1) / kSelThreads;
+  const int per = (n + NT - 1) / NT;
   const int i0 = min(n, tid * per), i1 = min(n, i0 + per);
   int gt = 0, eq = 0;
   for (int i = i0; i < i1; ++i) {
-    gt += keys[i] > prefix;
-    eq += keys[i] == prefix;
+    const uint32_t k = keys[i] & mask;
+    gt += k > prefix;
+    eq += k == prefix;
   }
-  // exclusive prefixes of both counts over the CTA (n < 2^16: packed in one word)
+  // exclusive prefixes of both counts over the CTA (gt < 2^11, eq < 2^16: packed in one word)
   const int pack = (gt << 16) | eq;
   int inc = pack;
 #pragma unroll
@@ -523,23 +730,23 @@ __global__ void __launch_bounds__(kSelThreads) block_select_kernel(const BlockSe
   __syncthreads();
   int base = inc - pack;
 #pragma unroll
-  for (int w = 0; w < kSelThreads / 32; ++w)
+  for (int w = 0; w < NWARP; ++w)
     if (w < warp) base += wsum[w];
   int gt_before = base >> 16, eq_before = base & 0xffff;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = keys[i];
-    const bool sel = k > prefix || (k == prefix && eq_before < need);
-    if (sel) out[a.sink + gt_before + min(eq_before, need)] = lo + i;
-    gt_before += k > prefix;
-    eq_before += k == prefix;
-  }
-  for (int i = tid; i < a.sink; i += kSelThreads) out[i] = i;
-  for (int i = first_local + tid; i < npages; i += kSelThreads) out[a.sink + want + (i - first_local)] = i;
+  if (gt + eq > 0)
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t k = keys[i] & mask;
+      if (k > prefix || (k == prefix && eq_before < need)) out[a.sink + gt_before + min(eq_before, need)] = lo + i;
+      gt_before += k > prefix;
+      eq_before += k == prefix;
+    }
+  for (int i = tid; i < a.sink; i += NT) out[i] = i;
+  for (int i = first_local + tid; i < npages; i += NT) out[a.sink + want + (i - first_local)] = i;
 }
 
 template <int D, int FMT>
 cudaError_t append_launch(const BlockAppendArgs& a, cudaStream_t s) {
-  const dim3 grid((a.T + a.slab - 1) / a.slab, a.Hk + (a.Hq + a.Hk + kWarps - 1) / kWarps);
+  const dim3 grid((a.T + a.slab - 1) / a.slab, a.Hk + (a.Hq + a.Hk + a.heads - 1) / a.heads);
   block_append_kernel<D, FMT><<<grid, kWarps * 32, 0, s>>>(a);
   return cudaGetLastError();
 }
@@ -548,13 +755,45 @@ cudaError_t summarize_launch(const BlockAppendArgs& a, const int* pages, int n, 
   block_summarize_kernel<D, FMT><<<dim3(n, a.Hk), kWarps * 32, 0, s>>>(a, pages);
   return cudaGetLastError();
 }
+template <int D, bool R8, int NT, int PP, int RES>
+cudaError_t select_launch_v(const BlockSelectArgs& a, int cs, cudaStream_t s) {
+  const int smem = 16 * (2 * D + 64) + 4 * a.pt_stride;
+  auto k = block_select_kernel<D, R8, NT, PP, RES>;
+  if (smem > 48 * 1024)
+    IOB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.B) * cs, a.Hk);
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cs;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k, a, cs);
+}
+template <int D, bool R8>
+cudaError_t select_launch_r(const BlockSelectArgs& a, cudaStream_t s) {
+  // Thousands of lists (a prefill chunk): small CTAs, many on an SM, so that one's selection runs under another's
+  // scores.  Enough to fill the SMs: the same with larger CTAs.  Few: the candidates of a list are split over a
+  // cluster until the SMs have two CTAs each, as long as a CTA keeps 64 pages, with 16 loads in flight per thread.
+  // (The page table's width bounds the candidates.)  Measured with each of the three forms, many / some / few: 512
+  // groups x 8 heads x 544 pages of D = 128: 84 / 98 / 141 us; 32 x 16 x 512 pages of D = 512: 50 / 38 / 45 us;
+  // 1 x 8 x 3200 pages of D = 128: 56 / 32 / 10 us.
+  const int units = a.B * a.Hk;
+  const int var = units >= 148 * 8 ? 2 : units > 148 ? 1 : 0;
+  int cs = 1;
+  while (var == 0 && cs < 8 && units * cs * 2 <= 2 * 148 && a.pt_stride >= 128 * cs) cs *= 2;
+  if (var == 2) return select_launch_v<D, R8, 128, 1, 8>(a, cs, s);
+  if (var == 1) return select_launch_v<D, R8, 256, 1, 4>(a, cs, s);
+  return select_launch_v<D, R8, 256, 1024 / (2 * D), 2>(a, cs, s);
+}
 template <int D>
 cudaError_t select_launch(const BlockSelectArgs& a, cudaStream_t s) {
-  const int smem = 16 * (2 * D + 64) + 4 * a.pt_stride;
-  if (smem > 48 * 1024)
-    IOB_CUDA_CHECK(cudaFuncSetAttribute(block_select_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  block_select_kernel<D><<<dim3(a.B, a.Hk), kSelThreads, smem, s>>>(a);
-  return cudaGetLastError();
+  return a.n_q * (a.Hq / a.Hk) <= 8 ? select_launch_r<D, true>(a, s) : select_launch_r<D, false>(a, s);
 }
 
 #define IOB_BY_D_FMT(fn, ...)                                                     \
@@ -578,6 +817,7 @@ cudaError_t block_append(const BlockAppendArgs& a_, cudaStream_t s) {
   if (a.T == 0) return cudaSuccess;
   // A decode step (few rows, each its own page) wants a CTA per row; a prefill wants fewer, longer CTAs.
   a.slab = a.T <= 256 ? 1 : 16;
+  a.heads = 4;
   IOB_BY_D_FMT(append_launch, a, s)
 }
 

@@ -365,7 +365,8 @@ struct BlockAppendArgs {
   void* scale;          // bf16 [num_pages, Hk], powers of two; inf = a key was not finite
   int fmt;
   float k_scale, v_scale;
-  int T, Hq, Hk, D, slots, max_pos, slab;
+  int T, Hq, Hk, D, slots, max_pos;
+  int slab, heads;      // rows of a CTA, heads of a q / v CTA (set by the launcher)
   float eps;
   bool plus_one;
 };
