@@ -2,16 +2,19 @@
 // at most 16 rows) against the listed 64-token pages of its request, softmax over the visible positions of those
 // pages, output and log-sum-exp.
 //
-// One cluster of C CTAs per (group, kv head); the CTAs share the list, each runs a streaming softmax over its pages
-// (running maximum m, sum l and output O in fp32, one pass), and the partial results are joined over distributed
-// shared memory, so a list is one launch whatever its split.  A page's K and V arrive as one bulk copy into a ring of
-// stages.  Per tile: S = Q K^T (warps split the tokens, and from D = 256 on also the head dim), scores through shared
-// memory to a row-wise softmax, P back as the A operand, O += P V (warps split the head dim).
+// One cluster of C CTAs per (group, kv head).  The list is cut into tiles of ST tokens, dealt out in turn to the warps
+// of the cluster; every warp runs a streaming softmax over its tiles by itself (one pass, running maximum m, sum l
+// and output O in fp32 registers, no barrier) and the partial results are joined at the end, over distributed shared
+// memory between CTAs, so a list is one launch whatever its split.  A warp's K and V tiles arrive by bulk copies in a
+// ring of slots of its own.
 //
-// mma.sync m16n8k16 carries both products: a list of single-token queries has at most 16 rows, so the tensor work is
-// small against the bytes, and register operands let a page's 8-bit and 4-bit values be widened (exactly, to f16) on
-// their way from shared memory into the fragments.  K order inside a product is free, so a thread's 4 consecutive
-// bytes (E4M3: 4 values, E2M1: 8) are used as the fragment they arrive in, with Q's columns permuted alike.
+// Both products have the cache on the M side of mma.sync m16n8k16: S^T = K Q^T (16 tokens x 8 rows) and
+// O^T = V^T P^T (16 values x 8 rows), so a list of up to 8 query rows wastes no tensor row and holds half the
+// registers that rows on the M side would take (D = 512: 128 of output and 64 of Q).  P goes from the accumulator
+// layout to the operand layout by a register transpose.  The contraction index of a product may be permuted freely:
+// a thread's 4 consecutive bytes of K (E4M3: 4 values, E2M1: 8) are used as the fragment they arrive in, with Q's
+// columns permuted alike, and V's values as the row order of O^T they arrive in, undone when O is stored.  8-bit and
+// 4-bit values are widened to f16 (exactly, block scales included) between shared memory and the fragments.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -19,47 +22,50 @@ namespace iob {
 namespace {
 
 constexpr int kPage = 64;
-constexpr int kRows = 16;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr float kLog2e = 1.4426950408889634f;
+// The running maximum may lag behind the true one by this much in the base-2 exponentials: floating point keeps its
+// relative precision (P <= 2^8 in f16 as well), and the output is hardly ever rescaled after the first tiles.
+constexpr float kLag = 8.f;
 
-template <int D_, int FMT_>
+template <int D_, int FMT_, int NR_>
 struct Cfg {
-  static constexpr int D = D_, FMT = FMT_;
+  static constexpr int D = D_, FMT = FMT_, NR = NR_;       // NR: groups of 8 query rows
   static constexpr bool BF = FMT == kKvBf16;
-  static constexpr int NW = D == 128 ? 4 : 8;              // warps
-  static constexpr int NT = NW * 32;
-  static constexpr int DS = NW / 4;                        // head-dim splits of Q K^T (four token groups)
-  static constexpr int TT = (BF && D == 512) ? 32 : 64;    // tokens per tile
-  static constexpr int RB = BF ? 2 * D : FMT == kKvFp8 ? D : D / 2;
-  static constexpr int SC = FMT == kKvNvfp4 ? D / 16 : 0;  // scale bytes per row
-  static constexpr int PART = TT * (RB + SC);              // one of K, V of a tile
-  static constexpr int STAGE = 2 * PART;
-  static constexpr int NS = STAGE <= 20480 ? 4 : FMT == kKvNvfp4 ? 2 : 3;
+  static constexpr int RB = BF ? 2 * D : FMT == kKvFp8 ? D : D / 2;       // bytes of a row
+  static constexpr int SC = FMT == kKvNvfp4 ? D / 16 : 0;                 // block scale bytes of a row
+  static constexpr int ST = 4096 / RB < 16 ? 16 : 4096 / RB;              // tokens of a tile: 4 KB, at least 16
+  static constexpr int SUB = ST / 16;
+  static constexpr int TPP = kPage / ST;                   // tiles of a page
+  static constexpr int SLOT = ST * (RB + SC);              // K or V of a tile
+  static constexpr int PART = kPage * (RB + SC);           // K or V of a page
   static constexpr int NCH = RB / 16 < 8 ? RB / 16 : 8;    // chunk swizzle span of a row
-  static constexpr int SST = TT + (DS == 1 ? 8 : 16);      // floats between score rows
-  static constexpr int PST = TT + 8;                       // 16-bit values between P rows
-  static constexpr int KK = D / DS / 16;                   // k16 steps of a warp's share of Q K^T
-  static constexpr int N8 = TT / 32;                       // 8-token tiles of a token group
-  static constexpr int DW = D / NW;                        // output columns of a warp
-  static constexpr int NO = DW / 8;
-  static constexpr int off_s = NS * STAGE;
-  static constexpr int off_p = off_s + DS * kRows * SST * 4;
-  static constexpr int off_list = off_p + kRows * PST * 2;
+  static constexpr int NX = NCH / 2;
+  static constexpr int KK = D / 16;                        // k16 steps of Q K^T
+  static constexpr int MT = D / 16;                        // 16-value tiles of O^T
+  static constexpr int DP = D + 4;                         // floats between rows of a partial output
+  // CTAs of an SM: by registers (Q and O take D / 8 * NR + D / 4 * NR of a thread's), one less warp group where a slot
+  // is 16 KB
+  static constexpr int RES = SLOT > 8192 ? 1 : D * NR >= 512 ? 2 : D * NR >= 256 ? 3 : 4;
+  static constexpr int SMEM = 226 * 1024 / RES - 4096;     // of a CTA, beside its static part and a list of 64
+  static constexpr int NS = SMEM / (kWarps * SLOT) < 6 ? SMEM / (kWarps * SLOT) : 6;     // slots of a warp
+  static constexpr int RING = NS * SLOT;
+  static_assert(NS >= 2 && RING >= 8 * NR * DP * 4, "a warp's partial output takes the place of its ring");
+  static constexpr int off_list = kWarps * RING;
   static constexpr int smem(int cap) { return off_list + 8 * cap; }
-  // CTAs that share an SM: by shared memory, at most 4
-  static constexpr int RES = 230000 / (off_list + 3072) < 4 ? 230000 / (off_list + 3072) : 4;
 };
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+template <bool BF>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  if constexpr (BF)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -72,6 +78,11 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
@@ -92,365 +103,437 @@ __device__ __forceinline__ void e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   hi = e4m3x2_to_f16x2(static_cast<uint16_t>(w >> 16));
 }
 template <class C>
-__device__ __forceinline__ uint32_t swz(int row, int chunk) {       // byte offset of a row's 16-byte chunk in a part
+__device__ __forceinline__ uint32_t swz(int row, int chunk) {       // byte offset of a row's 16-byte chunk
   return row * C::RB + ((((chunk ^ row) & (C::NCH - 1)) | (chunk & ~(C::NCH - 1))) << 4);
 }
-
-// Two query values as one register of the A operand (bf16 as they are; f16 after the row's power of two).
+template <bool BF>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (BF) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+// Two query values as one register of an operand (bf16 as they are; f16 after the row's power of two).
 template <bool BF>
 __device__ __forceinline__ uint32_t q_pair(const __nv_bfloat16* q, float f) {
   if (!q) return 0u;
   const uint32_t raw = *reinterpret_cast<const uint32_t*>(q);
   if constexpr (BF) return raw;
-  const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&raw);
-  const __half2 h = __floats2half2_rn(__low2float(v) * f, __high2float(v) * f);
-  return *reinterpret_cast<const uint32_t*>(&h);
+  return pack16<false>(__uint_as_float(raw << 16) * f, __uint_as_float(raw & 0xffff0000u) * f);
+}
+
+// The list entries of one unit that name a page of the request and the pool, by one warp: logical pages in s_blk,
+// physical pages in s_phys; returns their number.
+__device__ __forceinline__ int valid_pages(const BlockDecodeArgs& a, int unit, int prow, int len, int* s_blk,
+                                           int* s_phys) {
+  const int lane = lane_id();
+  const int* list = a.blocks + static_cast<size_t>(unit) * a.budget;
+  int cnt = 0;
+  for (int i0 = 0; i0 < a.budget; i0 += 32) {
+    const int i = i0 + lane;
+    const int blk = i < a.budget ? list[i] : -1;
+    int phys = -1;
+    if (blk >= 0 && blk < a.pt_stride && blk * kPage < len)
+      phys = a.page_table[static_cast<size_t>(prow) * a.pt_stride + blk];
+    const bool ok = phys >= 0 && phys < a.pages;
+    const uint32_t m = __ballot_sync(0xffffffffu, ok);
+    if (ok) {
+      const int at = cnt + __popc(m & ((1u << lane) - 1));
+      s_blk[at] = blk;
+      s_phys[at] = phys;
+    }
+    cnt += __popc(m);
+  }
+  return cnt;
+}
+
+// Power of two that brings a query row into f16's range (one warp).
+template <int D>
+__device__ __forceinline__ float row_pow2(const __nv_bfloat16* q) {
+  float amax = 0.f;
+  if (q)
+    for (int d = 2 * lane_id(); d < D; d += 64) {
+      const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(q + d);
+      amax = fmaxf(amax, fmaxf(fabsf(__low2float(v)), fabsf(__high2float(v))));
+    }
+  amax = warp_max(amax);
+  int x = 0;
+  if (amax > 0.f && amax < INFINITY) frexpf(amax, &x);
+  x = max(-100, min(100, x));
+  return __int_as_float((x + 127) << 23);
 }
 
 template <class C>
-__global__ void __launch_bounds__(C::NT, C::RES) block_decode_kernel(const BlockDecodeArgs a, const int csize, const int cap) {
+__global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const BlockDecodeArgs a, const int csize,
+                                                                        const int cap, const int rgroups) {
+  constexpr int NR = C::NR, ROWS = 8 * NR;
   extern __shared__ __align__(1024) uint8_t sm[];
-  __shared__ __align__(8) uint64_t full[C::NS];
-  __shared__ float s_alpha[kRows], s_m[kRows], s_l[kRows], s_qf[kRows], s_f[8][kRows];
+  __shared__ __align__(8) uint64_t full[kWarps][C::NS];
+  __shared__ float s_wm[kWarps][ROWS], s_wl[kWarps][ROWS], s_m[ROWS], s_l[ROWS], s_qf[ROWS], s_f[8][ROWS];
   __shared__ int s_cnt, s_abort;
-  float* sS = reinterpret_cast<float*>(sm + C::off_s);
-  uint16_t* sP = reinterpret_cast<uint16_t*>(sm + C::off_p);
   int* s_blk = reinterpret_cast<int*>(sm + C::off_list);
   int* s_phys = s_blk + cap;
-
   const int tid = threadIdx.x, warp = warp_id(), lane = lane_id();
-  const int unit = blockIdx.x / csize, rank = blockIdx.x % csize;
+  const int rank = blockIdx.x % csize, ur = blockIdx.x / csize;
+  const int unit = ur / rgroups, r0 = (ur % rgroups) * ROWS;      // list, first query row of this cluster
   const int b = unit / a.Hk, h = unit % a.Hk;
-  const int G = a.Hq / a.Hk, R = a.n_q * G;
+  const int G = a.Hq / a.Hk, R = min(a.n_q * G - r0, ROWS);
   const int prow = a.req_idx ? a.req_idx[b] : b;
   const int len = (prow < 0 || prow >= a.rows) ? 0 : min(a.kv_len[b], a.pt_stride * kPage);
   const int q0 = len - a.n_q;                    // position of the group's first token (may be negative)
-
+  auto q_row = [&](int r) -> const __nv_bfloat16* {
+    if (r >= R) return nullptr;
+    return reinterpret_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(b * a.n_q + (r0 + r) / G) * a.q_stride +
+           static_cast<size_t>(h * G + (r0 + r) % G) * C::D;
+  };
   if (tid == 0) {
     s_abort = 0;
-    for (int i = 0; i < C::NS; ++i) mbar_init(&full[i], 1);
+    for (int i = 0; i < kWarps * C::NS; ++i) mbar_init(&full[0][0] + i, 1);
     fence_mbar_init();
   }
-  // ---- this CTA's pages: list entries rank, rank + csize, ...; entries outside the request or the pool drop out
   if (warp == 0) {
-    const int* list = a.blocks + static_cast<size_t>(unit) * a.budget;
-    int cnt = 0;
-    for (int i0 = rank; i0 < a.budget; i0 += 32 * csize) {
-      const int i = i0 + lane * csize;
-      const int blk = i < a.budget ? list[i] : -1;
-      int phys = -1;
-      if (blk >= 0 && blk < a.pt_stride && blk * kPage < len)
-        phys = a.page_table[static_cast<size_t>(prow) * a.pt_stride + blk];
-      const bool ok = phys >= 0 && phys < a.pages;
-      const uint32_t m = __ballot_sync(0xffffffffu, ok);
-      if (ok) {
-        const int at = cnt + __popc(m & ((1u << lane) - 1));
-        s_blk[at] = blk;
-        s_phys[at] = phys;
-      }
-      cnt += __popc(m);
-    }
+    const int cnt = valid_pages(a, unit, prow, len, s_blk, s_phys);
     if (lane == 0) s_cnt = cnt;
   } else if constexpr (!C::BF) {
-    // ---- powers of two that bring every query row into f16's range
-    for (int r = warp - 1; r < kRows; r += C::NW - 1) {
-      float amax = 0.f;
-      if (r < R) {
-        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) +
-                                 static_cast<size_t>(b * a.n_q + r / G) * a.q_stride + (h * G + r % G) * C::D;
-        for (int d = lane; d < C::D; d += 32) amax = fmaxf(amax, fabsf(__bfloat162float(q[d])));
-      }
-      amax = warp_max(amax);
-      int x = 0;
-      if (amax > 0.f && amax < INFINITY) frexpf(amax, &x);
-      x = max(-100, min(100, x));
-      if (lane == 0) s_qf[r] = __int_as_float((x + 127) << 23);
+    for (int r = warp - 1; r < ROWS; r += kWarps - 1) {
+      const float f = row_pow2<C::D>(q_row(r));
+      if (lane == 0) s_qf[r] = f;
     }
   }
   __syncthreads();
-  constexpr int TPP = kPage / C::TT;             // tiles per page
-  const int ntiles = s_cnt * TPP;
-  auto issue = [&](int tile) {                   // one thread
-    const int st = tile % C::NS;
-    const uint8_t* src = a.pool + (static_cast<size_t>(s_phys[tile / TPP]) * a.Hk + h) * (C::STAGE * TPP);
-    uint8_t* dst = sm + st * C::STAGE;
-    mbar_expect_tx(&full[st], C::STAGE);
-    if constexpr (TPP == 1) {
-      bulk_g2s(dst, src, C::STAGE, &full[st]);
+  // ---- this warp's tiles: t0, t0 + step, ...; slot q of its ring sequence holds K (q even) or V of tile q / 2
+  const int ntiles = s_cnt * C::TPP;
+  const int step = csize * kWarps, t0 = warp * csize + rank;
+  const int nk = ntiles > t0 ? (ntiles - t0 + step - 1) / step : 0;
+  uint8_t* ring = sm + warp * C::RING;
+  auto issue = [&](int q, int slot) {            // lane 0
+    const int tile = t0 + (q >> 1) * step;
+    const uint8_t* src = a.pool + (static_cast<size_t>(s_phys[tile / C::TPP]) * a.Hk + h) * (2 * C::PART) +
+                         (q & 1) * C::PART;
+    uint8_t* dst = ring + slot * C::SLOT;
+    mbar_expect_tx(&full[warp][slot], C::SLOT);
+    if constexpr (C::SC == 0 || C::TPP == 1) {
+      bulk_g2s(dst, src + (tile % C::TPP) * C::SLOT, C::SLOT, &full[warp][slot]);
     } else {
-      src += (tile % TPP) * C::PART;
-      bulk_g2s(dst, src, C::PART, &full[st]);
-      bulk_g2s(dst + C::PART, src + TPP * C::PART, C::PART, &full[st]);
+      bulk_g2s(dst, src + (tile % C::TPP) * (C::ST * C::RB), C::ST * C::RB, &full[warp][slot]);
+      bulk_g2s(dst + C::ST * C::RB, src + kPage * C::RB + (tile % C::TPP) * (C::ST * C::SC), C::ST * C::SC,
+               &full[warp][slot]);
     }
   };
-  if (tid == 0)
-    for (int i = 0; i < C::NS && i < ntiles; ++i) issue(i);
+  if (lane == 0)
+    for (int q = 0; q < C::NS && q < 2 * nk; ++q) issue(q, q);
 
-  // ---- Q fragments of this warp's head-dim share
-  const int g = lane >> 2, j4 = lane & 3;
-  const int tg = warp & 3, dh = warp >> 2;
-  uint32_t qf[C::KK][4];
-  {
-    const __nv_bfloat16* qr[2];
-    float f[2];
+  const int g = lane >> 2, j4 = lane & 3, mi = lane >> 3, ri = lane & 7;
+  // ---- Q: column n of an operand is query row 8 n + g
+  uint32_t qf[C::KK][NR][2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int r = g + 8 * k;
-      qr[k] = r < R ? reinterpret_cast<const __nv_bfloat16*>(a.q) +
-                          static_cast<size_t>(b * a.n_q + r / G) * a.q_stride + (h * G + r % G) * C::D +
-                          dh * (C::D / C::DS)
-                    : nullptr;
-      f[k] = C::BF ? 1.f : 1.f / s_qf[r];
-    }
+  for (int n = 0; n < NR; ++n) {
+    const __nv_bfloat16* q = q_row(8 * n + g);
+    const float f = C::BF ? 1.f : 1.f / s_qf[8 * n + g];
 #pragma unroll
     for (int kk = 0; kk < C::KK; ++kk) {
       int d0, d1;
       if constexpr (C::BF) { d0 = 16 * kk + 2 * j4; d1 = d0 + 8; }
       else if constexpr (C::FMT == kKvFp8) { d0 = 16 * kk + 4 * j4; d1 = d0 + 2; }
       else { d0 = 32 * (kk / 2) + 8 * j4 + 4 * (kk % 2); d1 = d0 + 2; }
-      qf[kk][0] = q_pair<C::BF>(qr[0] ? qr[0] + d0 : nullptr, f[0]);
-      qf[kk][1] = q_pair<C::BF>(qr[1] ? qr[1] + d0 : nullptr, f[1]);
-      qf[kk][2] = q_pair<C::BF>(qr[0] ? qr[0] + d1 : nullptr, f[0]);
-      qf[kk][3] = q_pair<C::BF>(qr[1] ? qr[1] + d1 : nullptr, f[1]);
+      qf[kk][n][0] = q_pair<C::BF>(q ? q + d0 : nullptr, f);
+      qf[kk][n][1] = q_pair<C::BF>(q ? q + d1 : nullptr, f);
     }
   }
-  // ---- softmax state: row srow is shared by TPR consecutive threads
-  constexpr int TPR = C::NT / kRows;
-  const int srow = tid / TPR, sc0 = 2 * (tid % TPR);
-  const int st_tok = srow < R ? srow / G : 0;
-  const float ks = C::BF ? 1.f : a.k_scale * s_qf[srow];
-  const float s_scale = a.sm_scale * ks * 1.4426950408889634f;
-  float m_run = -INFINITY, l_run = 0.f;
-  float acc[C::NO][4];
+  // ---- softmax state of this thread's rows 8 n + 2 j4 + e (shared by the 8 lanes of equal j4)
+  float scale[2 * NR], m[2 * NR], l[2 * NR];
 #pragma unroll
-  for (int i = 0; i < C::NO; ++i)
+  for (int i = 0; i < 2 * NR; ++i) {
+    const int r = 8 * (i >> 1) + 2 * j4 + (i & 1);
+    scale[i] = a.sm_scale * kLog2e * (C::BF ? 1.f : a.k_scale * s_qf[r]);
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+  }
+  float acc[C::MT][NR][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[i][k] = 0.f;
-  const uint32_t smb = smem_u32(sm);
+  for (int t = 0; t < C::MT; ++t)
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[t][n][k] = 0.f;
+  // Offsets of this lane's fragment rows: the chunk swizzle leaves NX of them (a load takes a pair of chunks), further
+  // pairs lie at constant distances.
+  uint32_t klane[C::NX], vlane[C::NX];
+#pragma unroll
+  for (int i = 0; i < C::NX; ++i) {
+    klane[i] = swz<C>((mi & 1) * 8 + ri, 2 * i + (mi >> 1));
+    vlane[i] = swz<C>((mi >> 1) * 8 + ri, 2 * i + (mi & 1));
+  }
 
-  for (int tile = 0; tile < ntiles; ++tile) {
-    const int st = tile % C::NS;
-    if (!mbar_wait(&full[st], (tile / C::NS) & 1, &s_abort, a.status, kTimeoutProducer)) s_abort = 1;
-    const uint32_t kb = smb + st * C::STAGE, vb = kb + C::PART;
-    const int base = s_blk[tile / TPP] * kPage + (tile % TPP) * C::TT;
-    // ---- S = Q K^T
-    float s[C::N8][4];
-#pragma unroll
-    for (int n = 0; n < C::N8; ++n)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) s[n][k] = 0.f;
+  int slot = 0, phase = 0;
+  for (int k = 0; k < nk; ++k) {
+    const int tile = t0 + k * step;
+    const int base = s_blk[tile / C::TPP] * kPage + (tile % C::TPP) * C::ST;
+    // ---- S^T = K Q^T
+    if (!mbar_wait(&full[warp][slot], phase, &s_abort, a.status, kTimeoutProducer)) s_abort = 1;
+    float s[C::SUB][NR][4];
     {
-      const int c0 = dh * (C::RB / 16 / C::DS);
-      const int mi = lane >> 3, ri = lane & 7;
+      const uint8_t* kp = ring + slot * C::SLOT;
+      const uint32_t kb = smem_u32(kp);
+#pragma unroll
+      for (int u = 0; u < C::SUB; ++u) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u][n][e] = 0.f;
+        const uint32_t kt = kb + u * 16 * C::RB;
+        if constexpr (C::BF) {
+#pragma unroll
+          for (int kk = 0; kk < C::KK; ++kk) {
+            uint32_t r[4];
+            ldsm4(r, kt + klane[kk % C::NX] + kk / C::NX * (C::NCH * 16));
+#pragma unroll
+            for (int n = 0; n < NR; ++n) mma<true>(s[u][n], r, qf[kk][n]);
+          }
+        } else if constexpr (C::FMT == kKvFp8) {
+#pragma unroll
+          for (int i = 0; i < C::KK / 2; ++i) {
+            uint32_t r[4];
+            ldsm4(r, kt + klane[i % C::NX] + i / C::NX * (C::NCH * 16));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t f[4];
+              e4m3x4(r[2 * e], f[0], f[2]);
+              e4m3x4(r[2 * e + 1], f[1], f[3]);
+#pragma unroll
+              for (int n = 0; n < NR; ++n) mma<false>(s[u][n], f, qf[2 * i + e][n]);
+            }
+          }
+        } else {
+          // block scales of the two tokens u * 16 + g (+ 8): of each pair of a chunk's bytes this thread uses one
+          const uint8_t* ksc = kp + C::ST * C::RB + (u * 16 + g) * C::SC;
+          const uint32_t selp = (j4 >> 1) * 0x1111u;
+#pragma unroll
+          for (int i = 0; i < C::KK / 4; ++i) {              // pairs of 32-value chunks
+            uint32_t r[4], sw[2];
+            sw[0] = *reinterpret_cast<const uint32_t*>(ksc + 4 * i);
+            sw[1] = *reinterpret_cast<const uint32_t*>(ksc + 8 * C::SC + 4 * i);
+            ldsm4(r, kt + klane[i % C::NX] + i / C::NX * (C::NCH * 16));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t v[2][4];
+#pragma unroll
+              for (int o = 0; o < 2; ++o) {
+                const uint32_t s2 = e4m3x2_to_f16x2(static_cast<uint16_t>(prmt(sw[o], 0u, selp + e * 0x2222u)));
+                e2m1x8_to_f16x2x4(r[2 * e + o], v[o]);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[o][x] = hmul2_u32(v[o][x], s2);
+              }
+#pragma unroll
+              for (int t = 0; t < 2; ++t) {
+                const uint32_t f[4] = {v[0][2 * t], v[1][2 * t], v[0][2 * t + 1], v[1][2 * t + 1]};
+#pragma unroll
+                for (int n = 0; n < NR; ++n) mma<false>(s[u][n], f, qf[4 * i + 2 * e + t][n]);
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0 && 2 * k + C::NS < 2 * nk && !s_abort) issue(2 * k + C::NS, slot);
+    if (++slot == C::NS) { slot = 0; phase ^= 1; }
+    // ---- softmax over the tile's tokens u * 16 + g (+ 8)
+    if (base + C::ST - 1 > q0) {                 // some row does not see all of them
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int vis = min(len, q0 + (r0 + 8 * n + 2 * j4 + e) / G + 1) - base - g;
+#pragma unroll
+          for (int u = 0; u < C::SUB; ++u) {
+            if (16 * u >= vis) s[u][n][e] = -INFINITY;
+            if (16 * u + 8 >= vis) s[u][n][2 + e] = -INFINITY;
+          }
+        }
+    }
+    float mt[2 * NR];
+    bool over = false;
+#pragma unroll
+    for (int i = 0; i < 2 * NR; ++i) {
+      float x = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < C::SUB; ++u) x = fmaxf(x, fmaxf(s[u][i >> 1][i & 1], s[u][i >> 1][2 + (i & 1)]));
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+      mt[i] = x;
+      over |= (x - m[i]) * scale[i] > kLag;      // (m = -inf: any finite score; a score of -inf never)
+    }
+    if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+      for (int i = 0; i < 2 * NR; ++i) {
+        const float mn = fmaxf(m[i], mt[i]);
+        const float al = mn == -INFINITY ? 1.f : ex2((m[i] - mn) * scale[i]);
+        m[i] = mn;
+        l[i] *= al;
+#pragma unroll
+        for (int t = 0; t < C::MT; ++t) {
+          acc[t][i >> 1][i & 1] *= al;
+          acc[t][i >> 1][2 + (i & 1)] *= al;
+        }
+      }
+    }
+    uint32_t p[C::SUB][NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const float c0 = m[2 * n] == -INFINITY ? 0.f : -m[2 * n] * scale[2 * n];
+      const float c1 = m[2 * n + 1] == -INFINITY ? 0.f : -m[2 * n + 1] * scale[2 * n + 1];
+#pragma unroll
+      for (int u = 0; u < C::SUB; ++u) {
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const float p0 = ex2(fmaf(s[u][n][2 * o], scale[2 * n], c0));
+          const float p1 = ex2(fmaf(s[u][n][2 * o + 1], scale[2 * n + 1], c1));
+          l[2 * n] += p0;
+          l[2 * n + 1] += p1;
+          p[u][n][o] = transpose8x8(pack16<C::BF>(p0, p1));      // rows 8 n + g, tokens 2 j4, 2 j4 + 1 of the octet
+        }
+      }
+    }
+    // ---- O^T += V^T P^T
+    if (!mbar_wait(&full[warp][slot], phase, &s_abort, a.status, kTimeoutProducer)) s_abort = 1;
+    uint8_t* vp = ring + slot * C::SLOT;
+    if (base + C::ST > len) {                    // rows past the cache's end may hold anything: cleared
+      constexpr int ZB = C::FMT == kKvNvfp4 ? C::SC : C::RB;      // (an FP4 row is zero when its scales are)
+      uint8_t* z = vp + (C::FMT == kKvNvfp4 ? C::ST * C::RB : 0);
+      for (int i = max(0, len - base) * ZB + 4 * lane; i < C::ST * ZB; i += 128) *reinterpret_cast<uint32_t*>(z + i) = 0u;
+      fence_proxy_async_smem();
+      __syncwarp();
+    }
+    const uint32_t vb = smem_u32(vp);
+#pragma unroll
+    for (int u = 0; u < C::SUB; ++u) {
+      const uint32_t vt = vb + u * 16 * C::RB;
       if constexpr (C::BF) {
 #pragma unroll
-        for (int kk = 0; kk < C::KK; kk += 2 / C::N8) {
+        for (int t = 0; t < C::MT; ++t) {
           uint32_t r[4];
-          if constexpr (C::N8 == 2) {
-            ldsm4(r, kb + swz<C>(tg * 16 + (mi >> 1) * 8 + ri, c0 + 2 * kk + (mi & 1)));
-            mma_bf16(s[0], qf[kk], r[0], r[1]);
-            mma_bf16(s[1], qf[kk], r[2], r[3]);
-          } else {
-            ldsm4(r, kb + swz<C>(tg * 8 + ri, c0 + 2 * kk + mi));
-            mma_bf16(s[0], qf[kk], r[0], r[1]);
-            mma_bf16(s[0], qf[kk + 1], r[2], r[3]);
-          }
+          ldsm4t(r, vt + vlane[t % C::NX] + t / C::NX * (C::NCH * 16));
+#pragma unroll
+          for (int n = 0; n < NR; ++n) mma<true>(acc[t][n], r, p[u][n]);
         }
       } else if constexpr (C::FMT == kKvFp8) {
 #pragma unroll
-        for (int kk = 0; kk < C::KK; kk += 2) {
-          uint32_t r[4], lo, hi;
-          ldsm4(r, kb + swz<C>(tg * 16 + (mi >> 1) * 8 + ri, c0 + kk + (mi & 1)));
+        for (int i = 0; i < C::MT / 2; ++i) {
+          uint32_t r[4];
+          ldsm4t(r, vt + vlane[i % C::NX] + i / C::NX * (C::NCH * 16));
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int e = 0; e < 2; ++e) {          // a 16-byte chunk: values 2 g (rows g) and 2 g + 1 (rows g + 8)
+            uint32_t f[4];
+            e4m3x4(prmt(r[e], 0u, 0x3120u), f[0], f[1]);
+            e4m3x4(prmt(r[2 + e], 0u, 0x3120u), f[2], f[3]);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              e4m3x4(r[2 * n + k], lo, hi);
-              mma_f16(s[n], qf[kk + k], lo, hi);
-            }
-        }
-      } else {
-        const uint8_t* ksc = sm + st * C::STAGE + kPage * C::RB;
-#pragma unroll
-        for (int cc = 0; cc < C::KK / 2; cc += 2) {
-          uint32_t r[4], v[4];
-          ldsm4(r, kb + swz<C>(tg * 16 + (mi >> 1) * 8 + ri, c0 + cc + (mi & 1)));
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const uint32_t sb = ksc[(tg * 16 + n * 8 + g) * C::SC + 2 * (c0 + cc + k) + (j4 >> 1)];
-              const uint32_t s2 = e4m3x2_to_f16x2(static_cast<uint16_t>(sb | (sb << 8)));
-              e2m1x8_to_f16x2x4(r[2 * n + k], v);
-              mma_f16(s[n], qf[2 * (cc + k)], hmul2_u32(v[0], s2), hmul2_u32(v[1], s2));
-              mma_f16(s[n], qf[2 * (cc + k) + 1], hmul2_u32(v[2], s2), hmul2_u32(v[3], s2));
-            }
-        }
-      }
-    }
-    float* srowp = sS + dh * kRows * C::SST;
-#pragma unroll
-    for (int n = 0; n < C::N8; ++n) {
-      const int col = (tg * C::N8 + n) * 8 + 2 * j4;
-      *reinterpret_cast<float2*>(srowp + g * C::SST + col) = make_float2(s[n][0], s[n][1]);
-      *reinterpret_cast<float2*>(srowp + (g + 8) * C::SST + col) = make_float2(s[n][2], s[n][3]);
-    }
-    __syncthreads();
-    // ---- softmax of the tile's scores; value rows past the cache's end are cleared (they may hold anything)
-    {
-      constexpr int NI = C::TT / (2 * TPR);
-      float2 x[NI];
-      float mt = -INFINITY;
-      const int vis = srow < R ? min(len, q0 + st_tok + 1) - base : 0;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int col = sc0 + i * 2 * TPR;
-        x[i] = *reinterpret_cast<const float2*>(sS + srow * C::SST + col);
-        if constexpr (C::DS == 2) {
-          const float2 y = *reinterpret_cast<const float2*>(sS + (kRows + srow) * C::SST + col);
-          x[i].x += y.x;
-          x[i].y += y.y;
-        }
-        x[i].x = col < vis ? x[i].x * s_scale : -INFINITY;
-        x[i].y = col + 1 < vis ? x[i].y * s_scale : -INFINITY;
-        mt = fmaxf(mt, fmaxf(x[i].x, x[i].y));
-      }
-#pragma unroll
-      for (int o = 1; o < TPR; o <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-      const float m_new = fmaxf(m_run, mt);
-      const float ms = m_new == -INFINITY ? 0.f : m_new;
-      const float al = ex2(m_run - ms);
-      m_run = m_new;
-      l_run *= al;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const float p0 = ex2(x[i].x - ms), p1 = ex2(x[i].y - ms);
-        l_run += p0 + p1;
-        uint32_t raw;
-        if constexpr (C::BF) {
-          const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);
-          raw = *reinterpret_cast<const uint32_t*>(&v);
-        } else {
-          const __half2 v = __floats2half2_rn(p0, p1);
-          raw = *reinterpret_cast<const uint32_t*>(&v);
-        }
-        *reinterpret_cast<uint32_t*>(sP + srow * C::PST + sc0 + i * 2 * TPR) = raw;
-      }
-      if (tid % TPR == 0) s_alpha[srow] = al;
-      if (base + C::TT > len) {
-        uint8_t* v = sm + st * C::STAGE + C::PART;
-        constexpr int ZB = C::FMT == kKvNvfp4 ? C::SC : C::RB;      // an FP4 row is zero when its scales are
-        uint8_t* z = v + (C::FMT == kKvNvfp4 ? C::TT * C::RB : 0);
-        for (int i = max(0, len - base) * ZB + 4 * tid; i < C::TT * ZB; i += 4 * C::NT)
-          *reinterpret_cast<uint32_t*>(z + i) = 0u;
-        fence_proxy_async_smem();
-      }
-    }
-    __syncthreads();
-    // ---- O = alpha O + P V
-    {
-      const float al0 = s_alpha[g], al1 = s_alpha[g + 8];
-#pragma unroll
-      for (int i = 0; i < C::NO; ++i) {
-        acc[i][0] *= al0;
-        acc[i][1] *= al0;
-        acc[i][2] *= al1;
-        acc[i][3] *= al1;
-      }
-      const uint32_t pb = smem_u32(sP) + ((lane & 15) * C::PST + (lane >> 4) * 8) * 2;
-      const int mi = lane >> 3, ri = lane & 7;
-      if constexpr (C::BF) {
-        const int c0 = warp * (C::DW / 8);
-#pragma unroll
-        for (int kt = 0; kt < C::TT / 16; ++kt) {
-          uint32_t p[4], r[4];
-          ldsm4(p, pb + kt * 32);
-#pragma unroll
-          for (int c = 0; c < C::NO; c += 2) {
-            ldsm4t(r, vb + swz<C>(kt * 16 + (mi & 1) * 8 + ri, c0 + c + (mi >> 1)));
-            mma_bf16(acc[c], p, r[0], r[1]);
-            mma_bf16(acc[c + 1], p, r[2], r[3]);
+            for (int n = 0; n < NR; ++n) mma<false>(acc[2 * i + e][n], f, p[u][n]);
           }
         }
       } else {
-        const int c0 = warp * (C::DW * C::RB / C::D / 16);
-        const uint8_t* vsc = sm + st * C::STAGE + C::PART + kPage * C::RB;
-        (void)vsc;
+        const uint8_t* vsc = vp + C::ST * C::RB + (u * 16 + 2 * j4) * C::SC;
 #pragma unroll
-        for (int kt = 0; kt < C::TT / 32; ++kt) {
-          uint32_t p[2][4], r[4];
-          ldsm4(p[0], pb + kt * 64);
-          ldsm4(p[1], pb + kt * 64 + 32);
+        for (int i = 0; i < C::MT / 4; ++i) {
+          uint32_t r[4], sv[2][2];               // [octet][token 2 j4, 2 j4 + 1]: scale bytes of the chunk pair
 #pragma unroll
-          for (int c = 0; c < C::DW * C::RB / C::D / 16; ++c) {
-            ldsm4t(r, vb + swz<C>(kt * 32 + mi * 8 + ri, c0 + c));
-            if constexpr (C::FMT == kKvFp8) {
-              uint32_t e[4], o[4];
+          for (int o = 0; o < 2; ++o)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) e4m3x4(prmt(r[k], 0u, 0x3120u), e[k], o[k]);
+            for (int e = 0; e < 2; ++e) sv[o][e] = *reinterpret_cast<const uint32_t*>(vsc + (8 * o + e) * C::SC + 4 * i);
+          ldsm4t(r, vt + vlane[i % C::NX] + i / C::NX * (C::NCH * 16));
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                mma_f16(acc[2 * c], p[k], e[2 * k], e[2 * k + 1]);
-                mma_f16(acc[2 * c + 1], p[k], o[2 * k], o[2 * k + 1]);
-              }
-            } else {
-              uint32_t v[4][4];                    // [token octet][value of the 4]
+          for (int e = 0; e < 2; ++e) {          // a chunk of 32 values: 4 g + {0 .. 3}
+            uint32_t v[2][4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int t0 = kt * 32 + k * 8 + 2 * j4, blk = 2 * (c0 + c) + (lane >> 4);
-                const uint32_t sb = vsc[t0 * C::SC + blk] | (static_cast<uint32_t>(vsc[(t0 + 1) * C::SC + blk]) << 8);
-                const uint32_t s2 = e4m3x2_to_f16x2(static_cast<uint16_t>(sb));
-                // nibbles of tokens t0 (low half) and t0 + 1 (high half) -> bytes of one value's token pair, in
-                // the low halves of two bit selections
-                const uint32_t ev = (r[k] & 0x0f0f0f0fu) | ((r[k] >> 12) & 0xf0f0f0f0u);       // values 0, 2
-                const uint32_t od = ((r[k] >> 4) & 0x0f0f0f0fu) | ((r[k] >> 16) & 0xf0f0f0f0u); // values 1, 3
-                uint32_t w[4];
-                e2m1x8_to_f16x2x4(prmt(ev, od, 0x5410u), w);                                    // 0, 2, 1, 3
-                v[k][0] = hmul2_u32(w[0], s2);
-                v[k][2] = hmul2_u32(w[1], s2);
-                v[k][1] = hmul2_u32(w[2], s2);
-                v[k][3] = hmul2_u32(w[3], s2);
-              }
+            for (int o = 0; o < 2; ++o) {
+              const uint32_t by = 2 * e + (lane >> 4);
+              const uint32_t s2 = e4m3x2_to_f16x2(static_cast<uint16_t>(prmt(sv[o][0], sv[o][1], by | (by + 4) << 4)));
+              uint32_t w[4];                     // (0, 1) (2, 3) of token 2 j4, then of 2 j4 + 1
+              e2m1x8_to_f16x2x4(r[2 * o + e], w);
+              v[o][0] = hmul2_u32(prmt(w[0], w[2], 0x5410u), s2);
+              v[o][1] = hmul2_u32(prmt(w[0], w[2], 0x7632u), s2);
+              v[o][2] = hmul2_u32(prmt(w[1], w[3], 0x5410u), s2);
+              v[o][3] = hmul2_u32(prmt(w[1], w[3], 0x7632u), s2);
+            }
 #pragma unroll
-              for (int k = 0; k < 2; ++k)
+            for (int t = 0; t < 2; ++t) {
+              const uint32_t f[4] = {v[0][2 * t], v[0][2 * t + 1], v[1][2 * t], v[1][2 * t + 1]};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mma_f16(acc[4 * c + e], p[k], v[2 * k][e], v[2 * k + 1][e]);
+              for (int n = 0; n < NR; ++n) mma<false>(acc[4 * i + 2 * e + t][n], f, p[u][n]);
             }
           }
         }
       }
     }
-    __syncthreads();
-    if (tid == 0 && tile + C::NS < ntiles && !s_abort) issue(tile + C::NS);
+    __syncwarp();
+    if (lane == 0 && 2 * k + 1 + C::NS < 2 * nk && !s_abort) issue(2 * k + 1 + C::NS, slot);
+    if (++slot == C::NS) { slot = 0; phase ^= 1; }
   }
-  // ---- partial results to shared memory (the ring is idle: every issued copy was waited for)
-  float* sO = reinterpret_cast<float*>(sm);            // [16][D]
+  // ---- partial result of the warp in place of its ring (idle: every issued copy was waited for)
+  float* wO = reinterpret_cast<float*>(ring);                     // [ROWS][DP]
 #pragma unroll
-  for (int o = 1; o < TPR; o <<= 1) l_run += __shfl_xor_sync(0xffffffffu, l_run, o);
-  if (tid % TPR == 0) {
-    s_m[srow] = m_run;
-    s_l[srow] = s_abort ? NAN : l_run;
-  }
+  for (int i = 0; i < 2 * NR; ++i) {
 #pragma unroll
-  for (int i = 0; i < C::NO; ++i) {
+    for (int o = 4; o < 32; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+    const int r = 8 * (i >> 1) + 2 * j4 + (i & 1);
+    if (g == 0) {
+      s_wm[warp][r] = m[i] * scale[i];
+      s_wl[warp][r] = s_abort ? NAN : l[i];
+    }
+    if (r < R) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int row = g + 8 * (k >> 1), e = k & 1;
-      int d;
-      if constexpr (C::BF) d = 8 * i + 2 * j4 + e;
-      else if constexpr (C::FMT == kKvFp8) d = 16 * (i / 2) + 4 * j4 + 2 * e + (i & 1);
-      else d = 32 * (i / 4) + 8 * j4 + 4 * e + (i & 3);
-      sO[row * C::D + warp * C::DW + d] = acc[i][k];
+      for (int t = 0; t < C::MT; ++t) {
+        int d, dn;                               // values of rows g, g + 8 of the tile
+        if constexpr (C::BF) { d = 16 * t + g; dn = 8; }
+        else if constexpr (C::FMT == kKvFp8) { d = 16 * t + 2 * g; dn = 1; }
+        else { d = 32 * (t >> 1) + 4 * g + 2 * (t & 1); dn = 1; }
+        wO[r * C::DP + d] = acc[t][i >> 1][i & 1];
+        wO[r * C::DP + d + dn] = acc[t][i >> 1][2 + (i & 1)];
+      }
     }
   }
+  __syncthreads();
+  // ---- the CTA's partial result, in place of warp 0's
+  if (tid < ROWS) {
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_wm[w][tid]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2(s_wm[w][tid] - (M == -INFINITY ? 0.f : M));
+      s_f[w][tid] = f;
+      L += f * s_wl[w][tid];
+    }
+    s_m[tid] = M;
+    s_l[tid] = L;
+  }
+  __syncthreads();
+  for (int i = tid; i < R * (C::D / 4); i += kThreads) {
+    const int row = i / (C::D / 4), at = 4 * (row * C::DP + 4 * (i % (C::D / 4)));
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = s_f[w][row];
+      const float4 v = *reinterpret_cast<const float4*>(sm + w * C::RING + at);
+      if (f != 0.f) {
+        o.x += f * v.x;
+        o.y += f * v.y;
+        o.z += f * v.z;
+        o.w += f * v.w;
+      }
+    }
+    *reinterpret_cast<float4*>(sm + at) = o;
+  }
+  // ---- join of the cluster: every CTA finishes its share of the R x D outputs
   if (csize > 1) cluster_sync_all();
   else __syncthreads();
-  // ---- join: every CTA finishes its share of the R x D outputs
-  const uint32_t am = smem_u32(s_m), al = smem_u32(s_l), ao = smem_u32(sO);
-  if (tid < kRows) {
+  const uint32_t am = smem_u32(s_m), al = smem_u32(s_l), ao = smem_u32(sm);
+  if (tid < ROWS) {
     float M = -INFINITY;
-    for (int c = 0; c < csize; ++c)
-      M = fmaxf(M, __uint_as_float(ld_cluster_u32(mapa_shared(am + 4 * tid, c))));
+    for (int c = 0; c < csize; ++c) M = fmaxf(M, __uint_as_float(ld_cluster_u32(mapa_shared(am + 4 * tid, c))));
     const float ms = M == -INFINITY ? 0.f : M;
     float L = 0.f;
     for (int c = 0; c < csize; ++c) {
@@ -461,17 +544,17 @@ __global__ void __launch_bounds__(C::NT, C::RES) block_decode_kernel(const Block
     const float inv = L == 0.f ? 0.f : (C::BF ? 1.f : a.v_scale) / L;
     for (int c = 0; c < csize; ++c) s_f[c][tid] *= inv;
     if (rank == 0 && tid < R)
-      a.lse[static_cast<size_t>(b * a.n_q + tid / G) * a.Hq + h * G + tid % G] =
+      a.lse[static_cast<size_t>(b * a.n_q + (r0 + tid) / G) * a.Hq + h * G + (r0 + tid) % G] =
           L == 0.f ? -INFINITY : 0.6931471805599453f * (M + log2f(L));
   }
   __syncthreads();
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out);
-  for (int i = rank * C::NT + tid; i < R * (C::D / 4); i += csize * C::NT) {
+  for (int i = rank * kThreads + tid; i < R * (C::D / 4); i += csize * kThreads) {
     const int row = i / (C::D / 4), d = 4 * (i % (C::D / 4));
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = 0; c < csize; ++c) {
       const float f = s_f[c][row];
-      const float4 v = ld_cluster_f4(mapa_shared(ao + 4 * (row * C::D + d), c));
+      const float4 v = ld_cluster_f4(mapa_shared(ao + 4 * (row * C::DP + d), c));
       if (f != 0.f) {
         o.x += f * v.x;
         o.y += f * v.y;
@@ -479,30 +562,29 @@ __global__ void __launch_bounds__(C::NT, C::RES) block_decode_kernel(const Block
         o.w += f * v.w;
       }
     }
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x, o.y), hi = __floats2bfloat162_rn(o.z, o.w);
     uint2 raw;
-    raw.x = *reinterpret_cast<const uint32_t*>(&lo);
-    raw.y = *reinterpret_cast<const uint32_t*>(&hi);
-    *reinterpret_cast<uint2*>(out + (static_cast<size_t>(b * a.n_q + row / G) * a.Hq + h * G + row % G) * C::D + d) = raw;
+    raw.x = pack16<true>(o.x, o.y);
+    raw.y = pack16<true>(o.z, o.w);
+    *reinterpret_cast<uint2*>(out + (static_cast<size_t>(b * a.n_q + (r0 + row) / G) * a.Hq + h * G + (r0 + row) % G) *
+                                        C::D + d) = raw;
   }
   if (csize > 1) cluster_sync_all();             // a CTA's partial results are read until here
 }
 
-template <int D, int FMT>
-cudaError_t launch(const BlockDecodeArgs& a, cudaStream_t s) {
-  using C = Cfg<D, FMT>;
-  // Few lists: each is split over a cluster until every SM holds the CTAs it has room for, as long as a CTA keeps
-  // two pages.
-  const int units = a.B * a.Hk;
+template <int D, int FMT, int NR>
+cudaError_t launch_r(const BlockDecodeArgs& a, int rgroups, cudaStream_t s) {
+  using C = Cfg<D, FMT, NR>;
+  // Few lists: each is split over a cluster, as far as the SMs have room for all its CTAs at once and a CTA keeps two
+  // pages.
+  const int units = a.B * a.Hk * rgroups;
   int cs = 1;
-  while (cs < 8 && units * cs * 2 <= 148 * C::RES && a.budget >= 4 * cs) cs *= 2;
-  const int cap = (a.budget + cs - 1) / cs;
-  const int smem = C::smem(cap);
+  while (cs < 8 && units * (cs + 1) <= 148 * C::RES && a.budget >= 2 * (cs + 1)) ++cs;
+  const int smem = C::smem(a.budget);
   auto k = block_decode_kernel<C>;
   IOB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(units) * cs);
-  cfg.blockDim = dim3(C::NT);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -512,15 +594,24 @@ cudaError_t launch(const BlockDecodeArgs& a, cudaStream_t s) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, a, cs, cap);
+  return cudaLaunchKernelEx(&cfg, k, a, cs, a.budget, rgroups);
+}
+
+template <int D, int FMT>
+cudaError_t launch(const BlockDecodeArgs& a, cudaStream_t s) {
+  // Up to 8 query rows: one column group.  More: two, or for D = 512, where a warp has no registers for two, two
+  // clusters that read the same pages.
+  if (a.n_q * (a.Hq / a.Hk) <= 8) return launch_r<D, FMT, 1>(a, 1, s);
+  if constexpr (D == 512) return launch_r<D, FMT, 1>(a, 2, s);
+  else return launch_r<D, FMT, 2>(a, 1, s);
 }
 
 }  // namespace
 
 cudaError_t block_decode(const BlockDecodeArgs& a, cudaStream_t s) {
   if (a.B == 0) return cudaSuccess;
-  if (a.Hk < 1 || a.Hq % a.Hk || a.n_q < 1 || a.n_q * (a.Hq / a.Hk) > kRows || a.budget < 1 ||
-      a.budget > kBlockMaxList)
+  if (a.Hk < 1 || a.Hq % a.Hk || a.n_q < 1 || a.n_q * (a.Hq / a.Hk) > 16 || a.budget < 1 || a.budget > kBlockMaxList ||
+      !(a.sm_scale > 0.f) || (a.fmt != kKvBf16 && !(a.k_scale > 0.f)))
     return cudaErrorInvalidValue;
   switch (a.D * 4 + a.fmt) {
     case 128 * 4 + kKvBf16: return launch<128, kKvBf16>(a, s);

@@ -417,6 +417,7 @@ void block_decode(const at::Tensor& q, const at::Tensor& pool, const at::Tensor&
                   reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0, "out like q, contiguous");
   TORCH_CHECK(lse.is_contiguous() && lse.dim() == 2 && lse.size(0) == q.size(0) && lse.size(1) == q.size(1),
               "lse [B * n_q, Hq]");
+  TORCH_CHECK(sm_scale > 0 && k_scale > 0, "the softmax scale and the pool's key scale must be positive");
   iob::BlockDecodeArgs a{};
   a.q = q.data_ptr();
   a.q_stride = q.stride(0);

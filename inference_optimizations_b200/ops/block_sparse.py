@@ -214,6 +214,8 @@ def block_decode(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
         return out, lse
     _check_groups(q, page_table, kv_len, n_q, hk)
     _check_pool(pool, None, None, fmt, hk, q.shape[2])
+    if not (sm_scale > 0 and k_scale > 0):
+        raise RuntimeError("the softmax scale and the pool's key scale must be positive")
     if tuple(blocks.shape[:2]) != (kv_len.shape[0], hk) or not 1 <= blocks.shape[2] <= MAX_LIST:
         raise RuntimeError(f"blocks [B, Hk, 1 .. {MAX_LIST}]")
     o, z = block_decode_ref(q, pool, page_table, kv_len, blocks, n_q, hk, fmt, sm_scale, k_scale, v_scale, req_idx)

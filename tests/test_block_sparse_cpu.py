@@ -136,6 +136,9 @@ def test_refusals():
         S.block_decode(q[-1:], pool, table, kv, torch.zeros(1, 2, 4, dtype=torch.int32), 1, 2, 1, 0.1)
     with pytest.raises(RuntimeError):
         S.block_summarize(pool, torch.tensor([1]), codes[:1], sc, 0, 2, 128)
+    for kw in (dict(sm_scale=0.0), dict(sm_scale=-0.1), dict(sm_scale=0.1, k_scale=0.0)):
+        with pytest.raises(RuntimeError):
+            S.block_decode(q[-1:], pool, table, kv, torch.zeros(1, 2, 4, dtype=torch.int32), 1, 2, 0, **kw)
 
 
 # ------------------------------------------------------------------------------------------------ engine
