@@ -35,7 +35,14 @@ struct Cfg {
   static constexpr bool BF = FMT == kKvBf16;
   static constexpr int RB = BF ? 2 * D : FMT == kKvFp8 ? D : D / 2;       // bytes of a row
   static constexpr int SC = FMT == kKvNvfp4 ? D / 16 : 0;                 // block scale bytes of a row
-  static constexpr int ST = 4096 / RB < 16 ? 16 : 4096 / RB;              // tokens of a tile: 4 KB, at least 16
+  // Bytes of a tile (at least 16 tokens, at most a page) and CTAs of an SM, which the registers bound (Q and O take
+  // D / 8 * NR + D / 4 * NR of a thread's).  Larger tiles spread a step's fixed cost, more CTAs hide latencies.
+  // Measured, 8 KB with 3 CTAs against 4 KB with 4 (D = 128, one column group): bf16 32 x 8 x 32 pages 43.5 / 45.3 us,
+  // E4M3 64 x 8 x 32 pages 60.0 / 50.0 us, FP4 the same lists 48.4 / 42.4 us; two column groups, bf16 512 x 8 x 32
+  // pages 319 / 483 us.  D = 512, FP4, 32 x 16 x 64 pages: 8 KB 280 us, 4 KB 319 us.
+  static constexpr bool SMALL = D == 128 && NR == 1 && !BF;
+  static constexpr int TB = SMALL ? 4096 : 8192;
+  static constexpr int ST = TB / RB < 16 ? 16 : TB / RB < 64 ? TB / RB : 64;
   static constexpr int SUB = ST / 16;
   static constexpr int TPP = kPage / ST;                   // tiles of a page
   static constexpr int SLOT = ST * (RB + SC);              // K or V of a tile
@@ -45,10 +52,8 @@ struct Cfg {
   static constexpr int KK = D / 16;                        // k16 steps of Q K^T
   static constexpr int MT = D / 16;                        // 16-value tiles of O^T
   static constexpr int DP = D + 4;                         // floats between rows of a partial output
-  // CTAs of an SM: by registers (Q and O take D / 8 * NR + D / 4 * NR of a thread's), one less warp group where a slot
-  // is 16 KB
-  static constexpr int RES = SLOT > 8192 ? 1 : D * NR >= 512 ? 2 : D * NR >= 256 ? 3 : 4;
-  static constexpr int SMEM = 226 * 1024 / RES - 4096;     // of a CTA, beside its static part and a list of 64
+  static constexpr int RES = SLOT > 12000 ? 1 : D * NR >= 512 ? 2 : SMALL ? 4 : 3;
+  static constexpr int SMEM = 227 * 1024 / RES - 3584;     // of a CTA, beside its static part and a list of 64
   static constexpr int NS = SMEM / (kWarps * SLOT) < 6 ? SMEM / (kWarps * SLOT) : 6;     // slots of a warp
   static constexpr int RING = NS * SLOT;
   static_assert(NS >= 2 && RING >= 8 * NR * DP * 4, "a warp's partial output takes the place of its ring");
@@ -209,22 +214,27 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   const int step = csize * kWarps, t0 = warp * csize + rank;
   const int nk = ntiles > t0 ? (ntiles - t0 + step - 1) / step : 0;
   uint8_t* ring = sm + warp * C::RING;
-  auto issue = [&](int q, int slot) {            // lane 0
-    const int tile = t0 + (q >> 1) * step;
-    const uint8_t* src = a.pool + (static_cast<size_t>(s_phys[tile / C::TPP]) * a.Hk + h) * (2 * C::PART) +
-                         (q & 1) * C::PART;
+  int itile = t0;                                // lane 0: the next tile to fetch, its K's place, which part is next
+  const uint8_t* isrc = nullptr;
+  bool ival = false;
+  auto issue = [&](int slot) {
     uint8_t* dst = ring + slot * C::SLOT;
     mbar_expect_tx(&full[warp][slot], C::SLOT);
-    if constexpr (C::SC == 0 || C::TPP == 1) {
-      bulk_g2s(dst, src + (tile % C::TPP) * C::SLOT, C::SLOT, &full[warp][slot]);
+    const int in = itile % C::TPP;
+    if (!ival) {
+      isrc = a.pool + (static_cast<size_t>(s_phys[itile / C::TPP]) * a.Hk + h) * (2 * C::PART) + in * (C::ST * C::RB);
     } else {
-      bulk_g2s(dst, src + (tile % C::TPP) * (C::ST * C::RB), C::ST * C::RB, &full[warp][slot]);
-      bulk_g2s(dst + C::ST * C::RB, src + kPage * C::RB + (tile % C::TPP) * (C::ST * C::SC), C::ST * C::SC,
-               &full[warp][slot]);
+      isrc += C::PART;
+      itile += step;
     }
+    ival = !ival;
+    bulk_g2s(dst, isrc, C::SC == 0 || C::TPP == 1 ? C::SLOT : C::ST * C::RB, &full[warp][slot]);
+    if constexpr (C::SC != 0 && C::TPP != 1)
+      bulk_g2s(dst + C::ST * C::RB, isrc + kPage * C::RB - in * (C::ST * (C::RB - C::SC)), C::ST * C::SC,
+               &full[warp][slot]);
   };
   if (lane == 0)
-    for (int q = 0; q < C::NS && q < 2 * nk; ++q) issue(q, q);
+    for (int q = 0; q < C::NS && q < 2 * nk; ++q) issue(q);
 
   const int g = lane >> 2, j4 = lane & 3, mi = lane >> 3, ri = lane & 7;
   // ---- Q: column n of an operand is query row 8 n + g
@@ -339,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
       }
     }
     __syncwarp();
-    if (lane == 0 && 2 * k + C::NS < 2 * nk && !s_abort) issue(2 * k + C::NS, slot);
+    if (lane == 0 && 2 * k + C::NS < 2 * nk && !s_abort) issue(slot);
     if (++slot == C::NS) { slot = 0; phase ^= 1; }
     // ---- softmax over the tile's tokens u * 16 + g (+ 8)
     if (base + C::ST - 1 > q0) {                 // some row does not see all of them
@@ -469,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
       }
     }
     __syncwarp();
-    if (lane == 0 && 2 * k + 1 + C::NS < 2 * nk && !s_abort) issue(2 * k + 1 + C::NS, slot);
+    if (lane == 0 && 2 * k + 1 + C::NS < 2 * nk && !s_abort) issue(slot);
     if (++slot == C::NS) { slot = 0; phase ^= 1; }
   }
   // ---- partial result of the warp in place of its ring (idle: every issued copy was waited for)
