@@ -286,15 +286,15 @@ void block_groups(const at::Tensor& q, const at::Tensor& page_table, const c10::
   }
 }
 
-void block_append(const at::Tensor& qkv, c10::optional<at::Tensor> q_norm, c10::optional<at::Tensor> k_norm,
-                  const at::Tensor& cos_sin, const at::Tensor& pos, const at::Tensor& slot, at::Tensor q_out,
-                  at::Tensor pool, at::Tensor codes, at::Tensor scale, int64_t fmt, double k_scale, double v_scale,
+// (Outputs that the caller does not give are allocated here: a third of the cost of allocating them in Python.)
+at::Tensor block_append(const at::Tensor& qkv, c10::optional<at::Tensor> q_norm, c10::optional<at::Tensor> k_norm,
+                  const at::Tensor& cos_sin, const at::Tensor& pos, const at::Tensor& slot,
+                  c10::optional<at::Tensor> q_given, at::Tensor pool, at::Tensor codes, at::Tensor scale, int64_t fmt, double k_scale, double v_scale,
                   int64_t Hq, int64_t Hk, int64_t D, double eps, bool plus_one) {
   req(qkv, at::kBFloat16, "qkv");
   req(cos_sin, at::kFloat, "cos_sin");
   req(pos, at::kInt, "pos");
   req(slot, at::kInt, "slot");
-  req(q_out, at::kBFloat16, "q_out");
   block_pool(pool, fmt, Hk, D);
   block_bounds(codes, scale, pool.size(0), Hk, D);
   TORCH_CHECK(Hq >= 1 && Hk >= 1, "head counts");
@@ -305,6 +305,9 @@ void block_append(const at::Tensor& qkv, c10::optional<at::Tensor> q_norm, c10::
                   reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) % 16 == 0, "cos_sin [positions, D], contiguous");
   TORCH_CHECK(pos.is_contiguous() && slot.is_contiguous() && pos.numel() == qkv.size(0) &&
                   slot.numel() == qkv.size(0), "pos and slot [T]");
+  const at::cuda::CUDAGuard g(qkv.device());
+  const at::Tensor q_out = q_given.has_value() ? *q_given : at::empty({qkv.size(0), Hq, D}, qkv.options());
+  req(q_out, at::kBFloat16, "q_out");
   TORCH_CHECK(q_out.is_contiguous() && q_out.dim() == 3 && q_out.size(0) == qkv.size(0) && q_out.size(1) == Hq &&
                   q_out.size(2) == D && reinterpret_cast<uintptr_t>(q_out.data_ptr()) % 16 == 0,
               "q_out [T, Hq, D], contiguous");
@@ -337,8 +340,8 @@ void block_append(const at::Tensor& qkv, c10::optional<at::Tensor> q_norm, c10::
   a.max_pos = static_cast<int>(cos_sin.size(0));
   a.eps = static_cast<float>(eps);
   a.plus_one = plus_one;
-  const at::cuda::CUDAGuard g(qkv.device());
   CHECK_CUDA_OK(iob::block_append(a, stream()));
+  return q_out;
 }
 
 void block_summarize(const at::Tensor& pool, const at::Tensor& pages, at::Tensor codes, at::Tensor scale, int64_t fmt,
@@ -360,17 +363,22 @@ void block_summarize(const at::Tensor& pool, const at::Tensor& pages, at::Tensor
   CHECK_CUDA_OK(iob::block_summarize(a, pages.data_ptr<int>(), static_cast<int>(pages.size(0)), stream()));
 }
 
-void block_select(const at::Tensor& q, const at::Tensor& codes, const at::Tensor& scale, const at::Tensor& page_table,
-                  c10::optional<at::Tensor> req_idx, const at::Tensor& kv_len, at::Tensor blocks, at::Tensor count,
-                  int64_t n_q, int64_t Hk, int64_t budget, int64_t sink, int64_t local) {
+std::tuple<at::Tensor, at::Tensor> block_select(const at::Tensor& q, const at::Tensor& codes, const at::Tensor& scale,
+                  const at::Tensor& page_table, c10::optional<at::Tensor> req_idx, const at::Tensor& kv_len,
+                  c10::optional<at::Tensor> blocks_given, c10::optional<at::Tensor> count_given, int64_t n_q,
+                  int64_t Hk, int64_t budget, int64_t sink, int64_t local) {
   block_groups(q, page_table, req_idx, kv_len, n_q, Hk);
   const int64_t D = q.size(2), B = kv_len.size(0);
   TORCH_CHECK(D == 128 || D == 256 || D == 512, "head_dim 128, 256 or 512, got ", num(D));
   block_bounds(codes, scale, codes.dim() > 0 ? codes.size(0) : 0, Hk, D);
-  req(blocks, at::kInt, "blocks");
-  req(count, at::kInt, "count");
   TORCH_CHECK(sink >= 0 && local >= 1 && budget >= sink + local + 1 && budget <= iob::kBlockMaxList,
               "budget must hold sink + local + 1 pages and at most ", num(iob::kBlockMaxList));
+  const at::cuda::CUDAGuard g(q.device());
+  const auto ints = kv_len.options();
+  const at::Tensor blocks = blocks_given.has_value() ? *blocks_given : at::empty({B, Hk, budget}, ints);
+  const at::Tensor count = count_given.has_value() ? *count_given : at::empty({B, Hk}, ints);
+  req(blocks, at::kInt, "blocks");
+  req(count, at::kInt, "count");
   TORCH_CHECK(blocks.is_contiguous() && blocks.dim() == 3 && blocks.size(0) == B && blocks.size(1) == Hk &&
                   blocks.size(2) == budget, "blocks [B, Hk, budget]");
   TORCH_CHECK(count.is_contiguous() && count.dim() == 2 && count.size(0) == B && count.size(1) == Hk, "count [B, Hk]");
@@ -396,18 +404,23 @@ void block_select(const at::Tensor& q, const at::Tensor& codes, const at::Tensor
   a.budget = static_cast<int>(budget);
   a.sink = static_cast<int>(sink);
   a.local = static_cast<int>(local);
-  const at::cuda::CUDAGuard g(q.device());
   CHECK_CUDA_OK(iob::block_select(a, stream()));
+  return {blocks, count};
 }
 
-void block_decode(const at::Tensor& q, const at::Tensor& pool, const at::Tensor& page_table,
-                  c10::optional<at::Tensor> req_idx, const at::Tensor& kv_len, const at::Tensor& blocks, at::Tensor out,
-                  at::Tensor lse, c10::optional<at::Tensor> status, int64_t n_q, int64_t Hk, int64_t fmt,
-                  double sm_scale, double k_scale, double v_scale) {
+std::tuple<at::Tensor, at::Tensor> block_decode(const at::Tensor& q, const at::Tensor& pool,
+                  const at::Tensor& page_table, c10::optional<at::Tensor> req_idx, const at::Tensor& kv_len,
+                  const at::Tensor& blocks, c10::optional<at::Tensor> out_given, c10::optional<at::Tensor> lse_given,
+                  c10::optional<at::Tensor> status, int64_t n_q, int64_t Hk, int64_t fmt, double sm_scale,
+                  double k_scale, double v_scale) {
   block_groups(q, page_table, req_idx, kv_len, n_q, Hk);
   const int64_t D = q.size(2), B = kv_len.size(0);
   block_pool(pool, fmt, Hk, D);
   req(blocks, at::kInt, "blocks");
+  const at::cuda::CUDAGuard g(q.device());
+  const at::Tensor out = out_given.has_value() ? *out_given : at::empty(q.sizes(), q.options());
+  const at::Tensor lse =
+      lse_given.has_value() ? *lse_given : at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
   req(out, at::kBFloat16, "out");
   req(lse, at::kFloat, "lse");
   TORCH_CHECK(blocks.is_contiguous() && blocks.dim() == 3 && blocks.size(0) == B && blocks.size(1) == Hk &&
@@ -446,8 +459,8 @@ void block_decode(const at::Tensor& q, const at::Tensor& pool, const at::Tensor&
   a.sm_scale = static_cast<float>(sm_scale);
   a.k_scale = static_cast<float>(k_scale);
   a.v_scale = static_cast<float>(v_scale);
-  const at::cuda::CUDAGuard g(q.device());
   CHECK_CUDA_OK(iob::block_decode(a, stream()));
+  return {out, lse};
 }
 
 void mla_decode(c10::optional<at::Tensor> q, at::Tensor q8, at::Tensor q_scale, const at::Tensor& pool,

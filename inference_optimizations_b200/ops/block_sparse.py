@@ -68,12 +68,11 @@ def block_append(qkv: torch.Tensor, q_norm: Optional[torch.Tensor], k_norm: Opti
     bounds.  A row with slot -1, or with a position outside the table, is not written (its q is zero in the latter
     case).  Rows of one page are adjacent and ascending in a call, and its earlier rows were written by earlier calls
     on the stream: the order in which a request's tokens arrive."""
-    if q_out is None:
-        q_out = torch.empty(qkv.shape[0], hq, d, dtype=torch.bfloat16, device=qkv.device)
     if qkv.is_cuda:
-        ext().block_append(qkv, q_norm, k_norm, cos_sin, pos, slot, q_out, pool, codes, scale, fmt, k_scale, v_scale,
-                           hq, hk, d, eps, plus_one)
-        return q_out
+        return ext().block_append(qkv, q_norm, k_norm, cos_sin, pos, slot, q_out, pool, codes, scale, fmt, k_scale,
+                                  v_scale, hq, hk, d, eps, plus_one)
+    if q_out is None:
+        q_out = torch.empty(qkv.shape[0], hq, d, dtype=torch.bfloat16)
     _check_pool(pool, codes, scale, fmt, hk, d)
     if qkv.dim() != 2 or qkv.shape[1] < (hq + 2 * hk) * d or cos_sin.shape[-1] != d:
         raise RuntimeError("block_append: qkv [T, (Hq + 2 Hk) D], cos_sin [positions, D]")
@@ -137,13 +136,13 @@ def block_select(q: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, page
     the first `sink` pages and the pages from `local` - 1 before the group's first token on (they need no bounds:
     the last one is unfinished); the rest of the budget goes to the pages with the highest scores.
     budget >= sink + local + 1 (a group may straddle two pages)."""
-    b = kv_len.shape[0]
-    blocks, count = out if out is not None else (
-        torch.empty(b, hk, budget, dtype=torch.int32, device=q.device),
-        torch.empty(b, hk, dtype=torch.int32, device=q.device))
     if q.is_cuda:
-        ext().block_select(q, codes, scale, page_table, req_idx, kv_len, blocks, count, n_q, hk, budget, sink, local)
-        return blocks, count
+        blocks, count = out if out is not None else (None, None)
+        return ext().block_select(q, codes, scale, page_table, req_idx, kv_len, blocks, count, n_q, hk, budget, sink,
+                                  local)
+    b = kv_len.shape[0]
+    blocks, count = out if out is not None else (torch.empty(b, hk, budget, dtype=torch.int32),
+                                                 torch.empty(b, hk, dtype=torch.int32))
     _check_groups(q, page_table, kv_len, n_q, hk)
     if sink < 0 or local < 1 or not sink + local + 1 <= budget <= MAX_LIST:
         raise RuntimeError(f"budget must hold sink + local + 1 pages and at most {MAX_LIST}")
@@ -204,14 +203,13 @@ def block_decode(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
     once; entries < 0, past kv_len or without a page of the pool are skipped.  What the cache holds past kv_len is
     never used, whatever it is.  k_scale / v_scale are ignored on bf16 pools.  status int32 [1]: a copy that did not
     arrive within the wait limit records a code there (and the group's output is NaN)."""
-    if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    if lse is None:
-        lse = torch.empty(q.shape[0], q.shape[1], dtype=torch.float32, device=q.device)
     if q.is_cuda:
-        ext().block_decode(q, pool, page_table, req_idx, kv_len, blocks, out, lse, status, n_q, hk, fmt, sm_scale,
-                           k_scale, v_scale)
-        return out, lse
+        return ext().block_decode(q, pool, page_table, req_idx, kv_len, blocks, out, lse, status, n_q, hk, fmt,
+                                  sm_scale, k_scale, v_scale)
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16)
+    if lse is None:
+        lse = torch.empty(q.shape[0], q.shape[1], dtype=torch.float32)
     _check_groups(q, page_table, kv_len, n_q, hk)
     _check_pool(pool, None, None, fmt, hk, q.shape[2])
     if not (sm_scale > 0 and k_scale > 0):
