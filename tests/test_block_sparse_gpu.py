@@ -523,3 +523,64 @@ def test_refusals(cuda):
             app(**k)
     with pytest.raises(RuntimeError):
         S.block_summarize(pool, i2.long(), codes, sc, 0, hk, d)
+
+
+# ------------------------------------------------------------------------------------------------ engine
+def _engine(**kw):
+    from inference_optimizations_b200.config import EngineConfig
+    from inference_optimizations_b200.engine.engine import Engine
+    kw = {**dict(model="tiny_gqa", device="cuda:0", kv_dtype="bf16", max_running=4, chunked_prefill=64,
+                 graph_batch_sizes="1,2,4"), **kw}
+    return Engine(EngineConfig(**kw), max_seq=1024)
+
+
+@pytest.mark.parametrize("spec", [False, True])
+def test_engine_with_room_for_every_page_follows_the_reference(cuda, spec):
+    from inference_optimizations_b200.engine.scheduler import SamplingParams
+    torch.manual_seed(0)
+    eng = _engine(sparse_pages=16, spec=spec)
+    prompts = [torch.randint(1, 500, (n,)).tolist() for n in (130, 17, 290)]
+    outs = eng.generate(prompts, SamplingParams(max_new_tokens=8))
+    checked = 0
+    for p, o in zip(prompts, outs):
+        seq = list(p)
+        for tok in o:
+            ref = eng.runner.model.reference_logits(seq)[-1]
+            top2 = torch.topk(ref, 2).values
+            if (top2[0] - top2[1]).item() <= 0.05:            # not a numerical tie
+                break
+            assert tok == int(ref.argmax())
+            checked += 1
+            seq.append(tok)
+    assert checked >= 8 and eng.runner.kv.sparse_status.item() == 0
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "nvfp4"])
+def test_engine_graphs_select_as_eager_steps_do(cuda, kv):
+    """A small budget: graph replays and eager steps give the same tokens, and the bounds of the pages that the
+    requests filled are those of the pool."""
+    from inference_optimizations_b200.engine.scheduler import SamplingParams
+    torch.manual_seed(2)
+    prompts = [torch.randint(1, 500, (n,)).tolist() for n in (700, 390, 65)]
+    outs = []
+    for graphs in (False, True):
+        eng = _engine(sparse_pages=4, kv_dtype=kv, cuda_graphs=graphs)
+        outs.append(eng.generate(prompts, SamplingParams(max_new_tokens=70)))
+        assert all(len(o) == 70 for o in outs[-1])
+        cache = eng.runner.kv
+        before = [(c.clone(), s.clone()) for c, s in (b for b in cache.bounds if b is not None)]
+        cache.summarize()
+        for (c, s), (c2, s2) in zip(before, (b for b in cache.bounds if b is not None)):
+            done = s.ne(0).all(1)
+            assert done.sum() >= 16 and torch.equal(c[done], c2[done]) and torch.equal(s[done], s2[done])
+    assert outs[0] == outs[1]
+
+
+def test_synthetic_long_sessions_decode(cuda):
+    from inference_optimizations_b200.engine.synthetic import synth_decode_sessions
+    eng = _engine(sparse_pages=4, kv_dtype="nvfp4")
+    reqs = synth_decode_sessions(eng, 3, 900, 8)
+    for _ in range(5):
+        eng.step()
+    assert all(len(r.output) >= 5 for r in reqs)
+    assert all(b[1].ne(0).all() for b in eng.runner.kv.bounds if b is not None)
