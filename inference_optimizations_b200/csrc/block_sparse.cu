@@ -528,31 +528,34 @@ __global__ void __launch_bounds__(NT, RES) block_select_kernel(const BlockSelect
   for (int r = warp; r < (R8 ? 8 : 16); r += NWARP) {
     const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) +
                              static_cast<size_t>(b * a.n_q + r / G) * a.q_stride + (h * G + r % G) * D;
-    constexpr int V = D / 32;             // consecutive values of a lane
-    float2 x[V / 2];
-    float amax = 0.f;
-    bool bad = false;
+    // Sizes compare as the bits of |bf16| do (inf and NaN above every number); rounding is to the nearest even, by an
+    // addition that leaves the whole number in the low byte.
+    constexpr int V = D / 32, P = V / 2;  // consecutive values of a lane
+    uint32_t raw[P] = {}, top = 0;
+    if (r < R) {
 #pragma unroll
-    for (int j = 0; j < V / 2; j += (V < 8 ? V / 2 : 4)) {
-      uint32_t raw[V < 8 ? V / 2 : 4] = {};
-      if (r < R) load_words<(V < 8 ? V / 2 : 4)>(q + lane * V + 2 * j, raw);
-#pragma unroll
-      for (int k = 0; k < (V < 8 ? V / 2 : 4); ++k) {
-        x[j + k] = bf2(raw[k]);
-        amax = fmaxf(amax, fmaxf(fabsf(x[j + k].x), fabsf(x[j + k].y)));
-        bad |= !(fabsf(x[j + k].x) < INFINITY && fabsf(x[j + k].y) < INFINITY);
-      }
+      for (int j = 0; j < P; j += (P < 4 ? P : 4)) load_words<(P < 4 ? P : 4)>(q + lane * V + 2 * j, &raw[j]);
     }
-    amax = warp_max(amax);
-    bad = __any_sync(0xffffffffu, bad);
-    const int e = code_exp(amax);
-    const float inv = pow2(-e);
-    uint32_t wc[V / 4] = {}, wa[V / 4] = {};
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = bad ? 0 : code8((j & 1) ? x[j / 2].y : x[j / 2].x, inv);
-      wc[j / 4] |= (static_cast<uint32_t>(c) & 0xffu) << (8 * (j & 3));
-      wa[j / 4] |= static_cast<uint32_t>(abs(c)) << (8 * (j & 3));
+    for (int j = 0; j < P; ++j) top = __vmaxu2(top, raw[j] & 0x7fff7fffu);
+    top = __reduce_max_sync(0xffffffffu, max(top >> 16, top & 0xffffu));
+    const bool bad = top >= 0x7f80u;
+    const int e = code_exp(__uint_as_float(top << 16));
+    const float inv = bad ? 0.f : pow2(-e), lim = bad ? 0.f : 127.f * pow2(e);
+    constexpr float kRound = 12582912.f;  // 1.5 x 2^23
+    uint32_t wc[V / 4], wa[V / 4];
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      uint32_t c[4], m[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 v = bf2(raw[(j + k) / 2]);
+        const float x = fminf(fmaxf((k & 1) ? v.y : v.x, -lim), lim);
+        c[k] = __float_as_uint(fmaf(x, inv, kRound));
+        m[k] = __float_as_uint(fmaf(fabsf(x), inv, kRound));
+      }
+      wc[j / 4] = prmt(prmt(c[0], c[1], 0x0040u), prmt(c[2], c[3], 0x0040u), 0x5410u);
+      wa[j / 4] = prmt(prmt(m[0], m[1], 0x0040u), prmt(m[2], m[3], 0x0040u), 0x5410u);
     }
     store_words<V / 4>(qs + r * RS + lane * V, wc);
     store_words<V / 4>(qs + r * RS + D + lane * V, wa);
@@ -587,18 +590,22 @@ __global__ void __launch_bounds__(NT, RES) block_select_kernel(const BlockSelect
     }
   }
   const float s0 = rscale[g], s1 = R8 ? -1.f : rscale[g + 8];
+  const int8_t* rec0 = a.codes + h * (2 * D) + 16 * j4;
+  const __nv_bfloat16* sc_h = reinterpret_cast<const __nv_bfloat16*>(a.scale) + h;
+  const uint32_t rec_stride = static_cast<uint32_t>(a.Hk) * (2 * D), hk = static_cast<uint32_t>(a.Hk);
+  const uint32_t pages = static_cast<uint32_t>(a.pages);
   const uint32_t key_addr = csize > 1 ? mapa_shared(smem_u32(keys), 0) : smem_u32(keys);
   for (int p0 = c0 + warp * PP * 8; p0 < c1; p0 += NWARP * PP * 8) {
     uint4 bv[PP][U];
     float sc[PP];
 #pragma unroll
     for (int i = 0; i < PP; ++i) {
-      const bool ok = phys[i] >= 0 && phys[i] < a.pages;
-      const size_t ph = static_cast<size_t>(ok ? phys[i] : 0) * a.Hk + h;
-      const uint4* rec = reinterpret_cast<const uint4*>(a.codes + ph * 2 * D) + j4;
+      const bool ok = static_cast<uint32_t>(phys[i]) < pages;
+      const uint32_t pg = ok ? static_cast<uint32_t>(phys[i]) : 0u;
+      const uint4* rec = reinterpret_cast<const uint4*>(rec0 + static_cast<uint64_t>(pg) * rec_stride);
 #pragma unroll
       for (int u = 0; u < U; ++u) bv[i][u] = rec[4 * u];
-      sc[i] = ok ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.scale)[ph]) : -1.f;
+      sc[i] = ok ? __bfloat162float(sc_h[static_cast<uint64_t>(pg) * hk]) : -1.f;
     }
     const int pn = p0 + NWARP * PP * 8;
 #pragma unroll
