@@ -298,6 +298,7 @@ at::Tensor block_append(const at::Tensor& qkv, c10::optional<at::Tensor> q_norm,
   block_pool(pool, fmt, Hk, D);
   block_bounds(codes, scale, pool.size(0), Hk, D);
   TORCH_CHECK(Hq >= 1 && Hk >= 1, "head counts");
+  TORCH_CHECK(qkv.size(0) <= 65535 * 16, "at most ", num(65535 * 16), " rows");
   TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) >= (Hq + 2 * Hk) * D, "qkv [T, (Hq + 2 Hk) D]");
   TORCH_CHECK(qkv.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
               "qkv rows must be 16-byte aligned");

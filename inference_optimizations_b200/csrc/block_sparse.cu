@@ -366,7 +366,8 @@ __device__ void finish_bound(const Bound<D, FMT>& bd, float unit, int8_t* codes,
 }
 
 // ------------------------------------------------------------------------------------------ append
-// Grid: x = slabs of `slab` rows; y < Hk: the K vectors of kv head y, else `heads` of the Hq + Hk q and v vectors.
+// Grid: y = slabs of `slab` rows; x < Hk: the K vectors of kv head x, else `heads` of the Hq + Hk q and v vectors (a
+// slab's CTAs run together: K's, which wait for their rows, beside those that only move bytes).
 // q and v: a warp takes a row and walks through the heads, the position's angles in registers and the next two heads'
 // values on their way.  K: a CTA owns the page runs that start in its slab (consecutive rows at consecutive slots of
 // one page): its warps share the run's rows, and when the run ends at the page's last row the CTA also reads the rows
@@ -381,14 +382,14 @@ template <int D, int FMT>
 __global__ void __launch_bounds__(kWarps * 32, D == 512 ? 5 : 6) block_append_kernel(const BlockAppendArgs a) {
   __shared__ uint32_t red[2][kWarps][D / 2];
   const int warp = warp_id(), lane = lane_id();
-  const int t0 = blockIdx.x * a.slab, t1 = min(a.T, t0 + a.slab);
+  const int t0 = blockIdx.y * a.slab, t1 = min(a.T, t0 + a.slab);
   const __nv_bfloat16* qkv = reinterpret_cast<const __nv_bfloat16*>(a.qkv);
   constexpr int part = FMT == kKvBf16 ? kPage * 2 * D : FMT == kKvFp8 ? kPage * D : kPage * (D / 2 + D / 16);
   float2 x[2 * Lane<D>::P], gain[2 * Lane<D>::P];
   Angles<D> an;
-  if (static_cast<int>(blockIdx.y) >= a.Hk) {
+  if (static_cast<int>(blockIdx.x) >= a.Hk) {
     // a warp per row where there are rows for it, else a warp per head
-    const int first = (blockIdx.y - a.Hk) * a.heads;
+    const int first = (blockIdx.x - a.Hk) * a.heads;
     const int vend = min(first + a.heads, a.Hq + a.Hk);
     const int v0 = first + (a.slab == 1 ? warp : 0), vstep = a.slab == 1 ? kWarps : 1;
     if (v0 >= vend) return;
@@ -426,14 +427,17 @@ __global__ void __launch_bounds__(kWarps * 32, D == 512 ? 5 : 6) block_append_ke
     }
     return;
   }
-  const int h = blockIdx.y;
+  const int h = blockIdx.x;
   const float unit = FMT == kKvBf16 ? 1.f : a.k_scale, inv = 1.f / unit;
   if (a.k_norm) load_gain<D>(a.k_norm, a.plus_one, lane, gain);
-  for (int t = t0; t < t1; ++t) {
-    const int s = row_slot(a, t);
-    if (s < 0) continue;
+  // rows of the slab (at most 32) that begin a run: every lane looks at one
+  const int ts = t0 + lane;
+  const int mine = ts < t1 ? row_slot(a, ts) : -1;
+  const bool begins = mine >= 0 && (ts == 0 || mine % kPage == 0 || row_slot(a, ts - 1) != mine - 1);
+  for (uint32_t todo = __ballot_sync(0xffffffffu, begins); todo != 0; todo &= todo - 1) {
+    const int first = __ffs(todo) - 1, t = t0 + first;
+    const int s = __shfl_sync(0xffffffffu, mine, first);
     const int page = s / kPage, off = s % kPage;
-    if (t > 0 && off != 0 && row_slot(a, t - 1) == s - 1) continue;              // inside a run that began before
     // rows of the run (at most to the page's end): every lane looks at two
     bool in0 = off + lane < kPage && t + lane < a.T, in1 = off + lane + 32 < kPage && t + lane + 32 < a.T;
     in0 = in0 && row_slot(a, t + lane) == s + lane;
@@ -753,7 +757,7 @@ __global__ void __launch_bounds__(NT, RES) block_select_kernel(const BlockSelect
 
 template <int D, int FMT>
 cudaError_t append_launch(const BlockAppendArgs& a, cudaStream_t s) {
-  const dim3 grid((a.T + a.slab - 1) / a.slab, a.Hk + (a.Hq + a.Hk + a.heads - 1) / a.heads);
+  const dim3 grid(a.Hk + (a.Hq + a.Hk + a.heads - 1) / a.heads, (a.T + a.slab - 1) / a.slab);
   block_append_kernel<D, FMT><<<grid, kWarps * 32, 0, s>>>(a);
   return cudaGetLastError();
 }
@@ -822,6 +826,7 @@ cudaError_t select_launch(const BlockSelectArgs& a, cudaStream_t s) {
 cudaError_t block_append(const BlockAppendArgs& a_, cudaStream_t s) {
   BlockAppendArgs a = a_;
   if (a.T == 0) return cudaSuccess;
+  if (a.T > 65535 * 16) return cudaErrorInvalidValue;      // the grid's second dimension
   // A decode step (few rows, each its own page) wants a CTA per row; a prefill wants fewer, longer CTAs.
   a.slab = a.T <= 256 ? 1 : 16;
   a.heads = 4;
