@@ -102,10 +102,25 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Four E4M3 bytes -> (bytes 0, 1) and (bytes 2, 3) as f16x2.
+// Exact conversions to f16 pairs, free to be scheduled.
+__device__ __forceinline__ uint32_t e4m3x2(uint32_t w) {            // low two bytes
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(w)));
+  return r;
+}
 __device__ __forceinline__ void e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  lo = e4m3x2_to_f16x2(static_cast<uint16_t>(w));
-  hi = e4m3x2_to_f16x2(static_cast<uint16_t>(w >> 16));
+  lo = e4m3x2(w);
+  hi = e4m3x2(w >> 16);
+}
+__device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&o)[4]) {      // byte k's two values -> o[k]
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}\n"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+      : "r"(w));
 }
 template <class C>
 __device__ __forceinline__ uint32_t swz(int row, int chunk) {       // byte offset of a row's 16-byte chunk
@@ -320,20 +335,21 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
         } else {
           // block scales of the two tokens u * 16 + g (+ 8): of each pair of a chunk's bytes this thread uses one
           const uint8_t* ksc = kp + C::ST * C::RB + (u * 16 + g) * C::SC;
-          const uint32_t selp = (j4 >> 1) * 0x1111u;
+          const uint32_t selp = (j4 >> 1) | (2 + (j4 >> 1)) << 4;
 #pragma unroll
           for (int i = 0; i < C::KK / 4; ++i) {              // pairs of 32-value chunks
             uint32_t r[4], sw[2];
             sw[0] = *reinterpret_cast<const uint32_t*>(ksc + 4 * i);
             sw[1] = *reinterpret_cast<const uint32_t*>(ksc + 8 * C::SC + 4 * i);
             ldsm4(r, kt + klane[i % C::NX] + i / C::NX * (C::NCH * 16));
+            const uint32_t sp[2] = {e4m3x2(prmt(sw[0], 0u, selp)), e4m3x2(prmt(sw[1], 0u, selp))};      // both chunks'
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               uint32_t v[2][4];
 #pragma unroll
               for (int o = 0; o < 2; ++o) {
-                const uint32_t s2 = e4m3x2_to_f16x2(static_cast<uint16_t>(prmt(sw[o], 0u, selp + e * 0x2222u)));
-                e2m1x8_to_f16x2x4(r[2 * e + o], v[o]);
+                const uint32_t s2 = prmt(sp[o], 0u, e ? 0x3232u : 0x1010u);
+                e2m1x8(r[2 * e + o], v[o]);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) v[o][x] = hmul2_u32(v[o][x], s2);
               }
@@ -454,15 +470,17 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
 #pragma unroll
             for (int e = 0; e < 2; ++e) sv[o][e] = *reinterpret_cast<const uint32_t*>(vsc + (8 * o + e) * C::SC + 4 * i);
           ldsm4t(r, vt + vlane[i % C::NX] + i / C::NX * (C::NCH * 16));
+          // scales of this lane's block in the two chunks, as pairs of the two tokens
+          const uint32_t pr[2] = {prmt(sv[0][0], sv[0][1], 0x6240u + (lane >> 4) * 0x1111u),
+                                  prmt(sv[1][0], sv[1][1], 0x6240u + (lane >> 4) * 0x1111u)};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {          // a chunk of 32 values: 4 g + {0 .. 3}
             uint32_t v[2][4];
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
-              const uint32_t by = 2 * e + (lane >> 4);
-              const uint32_t s2 = e4m3x2_to_f16x2(static_cast<uint16_t>(prmt(sv[o][0], sv[o][1], by | (by + 4) << 4)));
+              const uint32_t s2 = e4m3x2(e ? pr[o] >> 16 : pr[o]);
               uint32_t w[4];                     // (0, 1) (2, 3) of token 2 j4, then of 2 j4 + 1
-              e2m1x8_to_f16x2x4(r[2 * o + e], w);
+              e2m1x8(r[2 * o + e], w);
               v[o][0] = hmul2_u32(prmt(w[0], w[2], 0x5410u), s2);
               v[o][1] = hmul2_u32(prmt(w[0], w[2], 0x7632u), s2);
               v[o][2] = hmul2_u32(prmt(w[1], w[3], 0x5410u), s2);
