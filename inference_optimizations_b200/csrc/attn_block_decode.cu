@@ -26,7 +26,10 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 // The running maximum may lag behind the true one by this much in the base-2 exponentials: floating point keeps its
-// relative precision (P <= 2^8 in f16 as well), and the output is hardly ever rescaled after the first tiles.
+// relative precision (P <= 2^8 in f16 as well), and the output is hardly ever rescaled after the first tiles.  P is
+// rounded for the second product, to 11 bits (f16) or, over a bf16 cache, to 8: there the output is divided by the sum
+// of the rounded weights (a row of ones beside V), so that the rounding of a weight that dominates its row cancels; the
+// log-sum-exp takes the sum of the unrounded ones.
 constexpr float kLag = 8.f;
 
 template <int D_, int FMT_, int NR_>
@@ -192,7 +195,8 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   constexpr int NR = C::NR, ROWS = 8 * NR;
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ __align__(8) uint64_t full[kWarps][C::NS];
-  __shared__ float s_wm[kWarps][ROWS], s_wl[kWarps][ROWS], s_m[ROWS], s_l[ROWS], s_qf[ROWS], s_f[8][ROWS];
+  __shared__ float s_wm[kWarps][ROWS], s_wl[kWarps][ROWS], s_wn[kWarps][ROWS], s_m[ROWS], s_l[ROWS], s_n[ROWS],
+      s_qf[ROWS], s_f[8][ROWS];
   __shared__ int s_cnt, s_abort;
   int* s_blk = reinterpret_cast<int*>(sm + C::off_list);
   int* s_phys = s_blk + cap;
@@ -284,6 +288,12 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
     for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[t][n][k] = 0.f;
+  float accn[NR][4];                             // sum of the rounded weights, every row the same
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) accn[n][k] = 0.f;
+  constexpr uint32_t kOnes[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
   // Offsets of this lane's fragment rows: the chunk swizzle leaves NX of them (a load takes a pair of chunks), further
   // pairs lie at constant distances.
   uint32_t klane[C::NX], vlane[C::NX];
@@ -400,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
         const float al = mn == -INFINITY ? 1.f : ex2((m[i] - mn) * scale[i]);
         m[i] = mn;
         l[i] *= al;
+        accn[i >> 1][i & 1] *= al;
 #pragma unroll
         for (int t = 0; t < C::MT; ++t) {
           acc[t][i >> 1][i & 1] *= al;
@@ -439,6 +450,8 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
     for (int u = 0; u < C::SUB; ++u) {
       const uint32_t vt = vb + u * 16 * C::RB;
       if constexpr (C::BF) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) mma<true>(accn[n], kOnes, p[u][n]);
 #pragma unroll
         for (int t = 0; t < C::MT; ++t) {
           uint32_t r[4];
@@ -510,6 +523,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
     if (g == 0) {
       s_wm[warp][r] = m[i] * scale[i];
       s_wl[warp][r] = s_abort ? NAN : l[i];
+      s_wn[warp][r] = s_abort ? NAN : C::BF ? accn[i >> 1][i & 1] : l[i];
     }
     if (r < R) {
 #pragma unroll
@@ -526,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   __syncthreads();
   // ---- the CTA's partial result, in place of warp 0's
   if (tid < ROWS) {
-    float M = -INFINITY, L = 0.f;
+    float M = -INFINITY, L = 0.f, N = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_wm[w][tid]);
 #pragma unroll
@@ -534,9 +548,11 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
       const float f = ex2(s_wm[w][tid] - (M == -INFINITY ? 0.f : M));
       s_f[w][tid] = f;
       L += f * s_wl[w][tid];
+      N += f * s_wn[w][tid];
     }
     s_m[tid] = M;
     s_l[tid] = L;
+    s_n[tid] = N;
   }
   __syncthreads();
   for (int i = tid; i < R * (C::D / 4); i += kThreads) {
@@ -558,18 +574,19 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   // ---- join of the cluster: every CTA finishes its share of the R x D outputs
   if (csize > 1) cluster_sync_all();
   else __syncthreads();
-  const uint32_t am = smem_u32(s_m), al = smem_u32(s_l), ao = smem_u32(sm);
+  const uint32_t am = smem_u32(s_m), al = smem_u32(s_l), an = smem_u32(s_n), ao = smem_u32(sm);
   if (tid < ROWS) {
     float M = -INFINITY;
     for (int c = 0; c < csize; ++c) M = fmaxf(M, __uint_as_float(ld_cluster_u32(mapa_shared(am + 4 * tid, c))));
     const float ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
+    float L = 0.f, N = 0.f;
     for (int c = 0; c < csize; ++c) {
       const float f = ex2(__uint_as_float(ld_cluster_u32(mapa_shared(am + 4 * tid, c))) - ms);
       s_f[c][tid] = f;
       L += f * __uint_as_float(ld_cluster_u32(mapa_shared(al + 4 * tid, c)));
+      N += f * __uint_as_float(ld_cluster_u32(mapa_shared(an + 4 * tid, c)));
     }
-    const float inv = L == 0.f ? 0.f : (C::BF ? 1.f : a.v_scale) / L;
+    const float inv = L == 0.f ? 0.f : (C::BF ? 1.f : a.v_scale) / N;
     for (int c = 0; c < csize; ++c) s_f[c][tid] *= inv;
     if (rank == 0 && tid < R)
       a.lse[static_cast<size_t>(b * a.n_q + (r0 + tid) / G) * a.Hq + h * G + (r0 + tid) % G] =
