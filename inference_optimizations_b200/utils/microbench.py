@@ -4,6 +4,7 @@ captures run.  Usage:
     python -m inference_optimizations_b200.utils.microbench gqa_decode --b 8 --ctx 8192 --d 512 --fmt nvfp4
     python -m inference_optimizations_b200.utils.microbench mla_decode --b 64 --heads 128 --ctx 131072 --fmt nvfp4
     python -m inference_optimizations_b200.utils.microbench moe_gemm --b 64 --topk 8 --experts 32 --total-experts 256
+    python -m inference_optimizations_b200.utils.microbench block_sparse --b 32 --ctx 32768 --d 512 --topk 64
     python -m inference_optimizations_b200.utils.microbench hotops --only rmsnorm_fp8,router,kv_write --tokens 64,8192
 
 `--launches N` runs exactly N launches and no timing loop (the form used under ncu: `-s N-1 -c 1`).
@@ -87,6 +88,55 @@ def gqa_decode_case(b: int, hk: int, hq: int, d: int, ctx: int, fmt_name: str, n
     return {"kernel": "gqa_decode", "b": b, "hk": hk, "hq": hq, "d": d, "ctx": ctx, "fmt": fmt_name, "n_q": n_q,
             "window": window, "splits": list(splits), "us": round(us, 2), "bytes": nbytes,
             "gbs": round(nbytes / us / 1e3, 1), "frac_hbm": round(nbytes / us / 1e3 / PEAKS["hbm_gbs"], 3)}
+
+
+def block_sparse_case(b: int, hk: int, hq: int, d: int, ctx: int, fmt_name: str, n_q: int, pages: int,
+                      launches: int = 0) -> dict:
+    """One decode (or verify) step of block-sparse attention: append, page selection, attention over `pages` pages of
+    each request, against dense split-K decode of the same step."""
+    from ..engine.synthetic import fill_pool_random
+    from ..ops import attention as A
+    from ..ops import block_sparse as S
+    from ..ops import kvcache as K
+    from ..ops.basic import rope_table
+    dev = torch.device("cuda:0")
+    fmt = K.FMT_IDS[fmt_name]
+    per = (ctx + 63) // 64
+    pool = torch.empty(b * per + 1, hk, 2, K.part_bytes(fmt, d), dtype=torch.uint8, device=dev)
+    fill_pool_random(pool, fmt, d, 1)
+    codes, scale = S.alloc_bounds(pool.shape[0], hk, d, dev)
+    S.block_summarize(pool, torch.arange(pool.shape[0], dtype=torch.int32, device=dev), codes, scale, fmt, hk, d)
+    pt = (torch.randperm(b * per, device=dev) + 1).view(b, per).int()
+    kv_len = torch.full((b,), ctx, dtype=torch.int32, device=dev)
+    pos = (ctx - n_q + torch.arange(n_q, device=dev)).repeat(b).int()
+    slot = (pt.repeat_interleave(n_q, 0).gather(1, (pos // 64).long()[:, None])[:, 0] * 64 + pos % 64).int()
+    qkv = torch.randn(b * n_q, (hq + 2 * hk) * d, device=dev).to(torch.bfloat16)
+    cs = rope_table(ctx + 64, d, 1e6, dev)
+    sm = 1 / math.sqrt(d)
+
+    def append():
+        return S.block_append(qkv, None, None, cs, pos, slot, pool, codes, scale, fmt, hq, hk, d, 1e-6, True)
+    q = append()
+
+    def select():
+        return S.block_select(q, codes, scale, pt, kv_len, n_q, hk, pages)
+    blocks, _ = select()
+
+    def attend():
+        return S.block_decode(q, pool, pt, kv_len, blocks, n_q, hk, fmt, sm)
+    if launches:
+        for _ in range(launches):
+            append(), select(), attend()
+        torch.cuda.synchronize()
+        return {}
+    splits = A.split_policy(b * hk, ctx)
+    ws = A.DecodeWorkspace.allocate(b, hk, splits[0], d, device=dev)
+    res = {"append_us": _time(append), "select_us": _time(select), "attend_us": _time(attend),
+           "dense_us": _time(lambda: A.gqa_decode(q, pool, pt, kv_len, n_q, hk, fmt, sm, splits=splits, ws=ws))}
+    nbytes = {"select": b * per * hk * (2 * d + 2), "attend": b * min(pages, per) * hk * 2 * K.part_bytes(fmt, d)}
+    return {"kernel": "block_sparse", "b": b, "hk": hk, "hq": hq, "d": d, "ctx": ctx, "fmt": fmt_name, "n_q": n_q,
+            "pages": pages, **{k: round(v, 2) for k, v in res.items()},
+            **{f"{k}_gbs": round(v / res[f"{k}_us"] / 1e3, 1) for k, v in nbytes.items()}}
 
 
 def gqa_extend_case(chunk: int, ctx: int, hk: int, hq: int, d: int, fmt_name: str, window: int,
@@ -930,6 +980,8 @@ def main() -> None:
         dist.barrier()
         dist.destroy_process_group()
         r = {}
+    elif a.kernel == "block_sparse":
+        r = block_sparse_case(a.b, a.hk, a.hq, a.d, a.ctx, a.fmt, a.nq, a.topk, a.launches)
     elif a.kernel == "moe_gemm":
         r = moe_gemm_case(a.b, a.experts, a.total_experts, a.topk, a.hidden, a.ffn, a.wfmt, a.launches)
     elif a.kernel == "proj_gemms":
