@@ -55,12 +55,18 @@ struct Cfg {
   static constexpr int KK = D / 16;                        // k16 steps of Q K^T
   static constexpr int MT = D / 16;                        // 16-value tiles of O^T
   static constexpr int DP = D + 4;                         // floats between rows of a partial output
+  // Over FP4 caches Q's operand registers stay in shared memory where O takes 128 of a thread's: 64 more would leave
+  // too few to overlap the conversions (D = 512, 32 x 16 x 64 pages: 271 against 278 us; over 8-bit and 16-bit caches,
+  // bound by their bytes, registers are better: D = 512, bf16, 16 x 16 x 32 pages 151 against 144 us).
+  static constexpr bool QSM = D * NR >= 512 && FMT == kKvNvfp4;
+  static constexpr int QB = QSM ? KK * NR * 256 : 0;       // bytes of it
   static constexpr int RES = SLOT > 12000 ? 1 : D * NR >= 512 ? 2 : SMALL ? 4 : 3;
-  static constexpr int SMEM = 227 * 1024 / RES - 3584;     // of a CTA, beside its static part and a list of 64
+  static constexpr int SMEM = 227 * 1024 / RES - 3584 - QB;     // of a CTA's rings, beside its static part and a list of 64
   static constexpr int NS = SMEM / (kWarps * SLOT) < 6 ? SMEM / (kWarps * SLOT) : 6;     // slots of a warp
   static constexpr int RING = NS * SLOT;
   static_assert(NS >= 2 && RING >= 8 * NR * DP * 4, "a warp's partial output takes the place of its ring");
-  static constexpr int off_list = kWarps * RING;
+  static constexpr int off_q = kWarps * RING;
+  static constexpr int off_list = off_q + QB;
   static constexpr int smem(int cap) { return off_list + 8 * cap; }
 };
 
@@ -257,21 +263,39 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
 
   const int g = lane >> 2, j4 = lane & 3, mi = lane >> 3, ri = lane & 7;
   // ---- Q: column n of an operand is query row 8 n + g
-  uint32_t qf[C::KK][NR][2];
+  uint32_t qf[C::QSM ? 1 : C::KK][NR][2];
+  uint2* s_q = reinterpret_cast<uint2*>(sm + C::off_q) + lane;      // [KK][NR][32]
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     const __nv_bfloat16* q = q_row(8 * n + g);
     const float f = C::BF ? 1.f : 1.f / s_qf[8 * n + g];
 #pragma unroll
     for (int kk = 0; kk < C::KK; ++kk) {
+      if (C::QSM && kk % kWarps != warp) continue;                  // shared: each warp prepares its part
       int d0, d1;
       if constexpr (C::BF) { d0 = 16 * kk + 2 * j4; d1 = d0 + 8; }
       else if constexpr (C::FMT == kKvFp8) { d0 = 16 * kk + 4 * j4; d1 = d0 + 2; }
       else { d0 = 32 * (kk / 2) + 8 * j4 + 4 * (kk % 2); d1 = d0 + 2; }
-      qf[kk][n][0] = q_pair<C::BF>(q ? q + d0 : nullptr, f);
-      qf[kk][n][1] = q_pair<C::BF>(q ? q + d1 : nullptr, f);
+      const uint32_t x = q_pair<C::BF>(q ? q + d0 : nullptr, f), y = q_pair<C::BF>(q ? q + d1 : nullptr, f);
+      if constexpr (C::QSM) {
+        s_q[(kk * NR + n) * 32] = make_uint2(x, y);
+      } else {
+        qf[kk][n][0] = x;
+        qf[kk][n][1] = y;
+      }
     }
   }
+  if constexpr (C::QSM) __syncthreads();
+  auto q_at = [&](int kk, int n, uint32_t (&o)[2]) {
+    if constexpr (C::QSM) {
+      const uint2 v = s_q[(kk * NR + n) * 32];
+      o[0] = v.x;
+      o[1] = v.y;
+    } else {
+      o[0] = qf[kk][n][0];
+      o[1] = qf[kk][n][1];
+    }
+  };
   // ---- softmax state of this thread's rows 8 n + 2 j4 + e (shared by the 8 lanes of equal j4)
   float scale[2 * NR], m[2 * NR], l[2 * NR];
 #pragma unroll
@@ -314,25 +338,28 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
       const uint8_t* kp = ring + slot * C::SLOT;
       const uint32_t kb = smem_u32(kp);
 #pragma unroll
-      for (int u = 0; u < C::SUB; ++u) {
+      for (int u = 0; u < C::SUB; ++u)
 #pragma unroll
         for (int n = 0; n < NR; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[u][n][e] = 0.f;
-        const uint32_t kt = kb + u * 16 * C::RB;
-        if constexpr (C::BF) {
+      if constexpr (C::BF) {
+#pragma unroll
+        for (int u = 0; u < C::SUB; ++u)
 #pragma unroll
           for (int kk = 0; kk < C::KK; ++kk) {
             uint32_t r[4];
-            ldsm4(r, kt + klane[kk % C::NX] + kk / C::NX * (C::NCH * 16));
+            ldsm4(r, kb + u * 16 * C::RB + klane[kk % C::NX] + kk / C::NX * (C::NCH * 16));
 #pragma unroll
             for (int n = 0; n < NR; ++n) mma<true>(s[u][n], r, qf[kk][n]);
           }
-        } else if constexpr (C::FMT == kKvFp8) {
+      } else if constexpr (C::FMT == kKvFp8) {
+#pragma unroll
+        for (int u = 0; u < C::SUB; ++u)
 #pragma unroll
           for (int i = 0; i < C::KK / 2; ++i) {
             uint32_t r[4];
-            ldsm4(r, kt + klane[i % C::NX] + i / C::NX * (C::NCH * 16));
+            ldsm4(r, kb + u * 16 * C::RB + klane[i % C::NX] + i / C::NX * (C::NCH * 16));
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               uint32_t f[4];
@@ -342,33 +369,41 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
               for (int n = 0; n < NR; ++n) mma<false>(s[u][n], f, qf[2 * i + e][n]);
             }
           }
-        } else {
-          // block scales of the two tokens u * 16 + g (+ 8): of each pair of a chunk's bytes this thread uses one
-          const uint8_t* ksc = kp + C::ST * C::RB + (u * 16 + g) * C::SC;
-          const uint32_t selp = (j4 >> 1) | (2 + (j4 >> 1)) << 4;
+      } else {
+        // block scales of the two tokens u * 16 + g (+ 8): of each pair of a chunk's bytes this thread uses one
+        const uint8_t* ksc = kp + C::ST * C::RB + g * C::SC;
+        const uint32_t selp = (j4 >> 1) | (2 + (j4 >> 1)) << 4;
+        constexpr int NP = C::KK / 4;                        // pairs of 32-value chunks
+        uint32_t q[4][NR][2];                                // (shared Q: read once for all the tile's tokens)
 #pragma unroll
-          for (int i = 0; i < C::KK / 4; ++i) {              // pairs of 32-value chunks
-            uint32_t r[4], sw[2];
-            sw[0] = *reinterpret_cast<const uint32_t*>(ksc + 4 * i);
-            sw[1] = *reinterpret_cast<const uint32_t*>(ksc + 8 * C::SC + 4 * i);
-            ldsm4(r, kt + klane[i % C::NX] + i / C::NX * (C::NCH * 16));
-            const uint32_t sp[2] = {e4m3x2(prmt(sw[0], 0u, selp)), e4m3x2(prmt(sw[1], 0u, selp))};      // both chunks'
+        for (int it = 0; it < NP * C::SUB; ++it) {
+          const int u = C::QSM ? it % C::SUB : it / NP, i = C::QSM ? it / C::SUB : it % NP;
+          if (!C::QSM || u == 0) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              uint32_t v[2][4];
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
-              for (int o = 0; o < 2; ++o) {
-                const uint32_t s2 = prmt(sp[o], 0u, e ? 0x3232u : 0x1010u);
-                e2m1x8(r[2 * e + o], v[o]);
+              for (int n = 0; n < NR; ++n) q_at(4 * i + x, n, q[x][n]);
+          }
+          uint32_t r[4], sw[2];
+          sw[0] = *reinterpret_cast<const uint32_t*>(ksc + u * 16 * C::SC + 4 * i);
+          sw[1] = *reinterpret_cast<const uint32_t*>(ksc + (u * 16 + 8) * C::SC + 4 * i);
+          ldsm4(r, kb + u * 16 * C::RB + klane[i % C::NX] + i / C::NX * (C::NCH * 16));
+          const uint32_t sp[2] = {e4m3x2(prmt(sw[0], 0u, selp)), e4m3x2(prmt(sw[1], 0u, selp))};      // both chunks'
 #pragma unroll
-                for (int x = 0; x < 4; ++x) v[o][x] = hmul2_u32(v[o][x], s2);
-              }
+          for (int e = 0; e < 2; ++e) {
+            uint32_t v[2][4];
 #pragma unroll
-              for (int t = 0; t < 2; ++t) {
-                const uint32_t f[4] = {v[0][2 * t], v[1][2 * t], v[0][2 * t + 1], v[1][2 * t + 1]};
+            for (int o = 0; o < 2; ++o) {
+              const uint32_t s2 = prmt(sp[o], 0u, e ? 0x3232u : 0x1010u);
+              e2m1x8(r[2 * e + o], v[o]);
 #pragma unroll
-                for (int n = 0; n < NR; ++n) mma<false>(s[u][n], f, qf[4 * i + 2 * e + t][n]);
-              }
+              for (int x = 0; x < 4; ++x) v[o][x] = hmul2_u32(v[o][x], s2);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const uint32_t f[4] = {v[0][2 * t], v[1][2 * t], v[0][2 * t + 1], v[1][2 * t + 1]};
+#pragma unroll
+              for (int n = 0; n < NR; ++n) mma<false>(s[u][n], f, q[2 * e + t][n]);
             }
           }
         }
