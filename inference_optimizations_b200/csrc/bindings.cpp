@@ -299,6 +299,7 @@ at::Tensor block_append(const at::Tensor& qkv, c10::optional<at::Tensor> q_norm,
   block_bounds(codes, scale, pool.size(0), Hk, D);
   TORCH_CHECK(Hq >= 1 && Hk >= 1, "head counts");
   TORCH_CHECK(qkv.size(0) <= 65535 * 16, "at most ", num(65535 * 16), " rows");
+  TORCH_CHECK(fmt == iob::kKvBf16 || (k_scale > 0 && v_scale > 0), "the pool's scales must be positive");
   TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) >= (Hq + 2 * Hk) * D, "qkv [T, (Hq + 2 Hk) D]");
   TORCH_CHECK(qkv.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
               "qkv rows must be 16-byte aligned");
@@ -351,6 +352,7 @@ void block_summarize(const at::Tensor& pool, const at::Tensor& pages, at::Tensor
   block_bounds(codes, scale, pool.size(0), Hk, D);
   req(pages, at::kInt, "pages");
   TORCH_CHECK(pages.dim() == 1 && pages.is_contiguous(), "pages [n]");
+  TORCH_CHECK(fmt == iob::kKvBf16 || k_scale > 0, "the pool's scale must be positive");
   iob::BlockAppendArgs a{};
   a.pool = pool.data_ptr<uint8_t>();
   a.codes = reinterpret_cast<int8_t*>(codes.data_ptr());
@@ -431,7 +433,8 @@ std::tuple<at::Tensor, at::Tensor> block_decode(const at::Tensor& q, const at::T
                   reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0, "out like q, contiguous");
   TORCH_CHECK(lse.is_contiguous() && lse.dim() == 2 && lse.size(0) == q.size(0) && lse.size(1) == q.size(1),
               "lse [B * n_q, Hq]");
-  TORCH_CHECK(sm_scale > 0 && k_scale > 0, "the softmax scale and the pool's key scale must be positive");
+  TORCH_CHECK(sm_scale > 0 && (fmt == iob::kKvBf16 || k_scale > 0),
+              "the softmax scale and the pool's key scale must be positive");
   iob::BlockDecodeArgs a{};
   a.q = q.data_ptr();
   a.q_stride = q.stride(0);

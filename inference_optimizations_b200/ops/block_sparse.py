@@ -66,7 +66,7 @@ def block_append(qkv: torch.Tensor, q_norm: Optional[torch.Tensor], k_norm: Opti
     [T, Hq, D] (returned), k and v -> pool[slot] in the pool's format; everything in fp32 with one rounding at the end
     (`gqa_prep` rounds to bf16 after the norm).  Every page whose last row (slot % 64 == 63) is written gets its key
     bounds.  A row with slot -1, or with a position outside the table, is not written (its q is zero in the latter
-    case).  Rows of one page are adjacent and ascending in a call, and its earlier rows were written by earlier calls
+    case).  E4M3 values saturate.  Rows of one page are adjacent and ascending in a call, and its earlier rows were written by earlier calls
     on the stream: the order in which a request's tokens arrive."""
     if qkv.is_cuda:
         return ext().block_append(qkv, q_norm, k_norm, cos_sin, pos, slot, q_out, pool, codes, scale, fmt, k_scale,
@@ -76,6 +76,8 @@ def block_append(qkv: torch.Tensor, q_norm: Optional[torch.Tensor], k_norm: Opti
     _check_pool(pool, codes, scale, fmt, hk, d)
     if qkv.dim() != 2 or qkv.shape[1] < (hq + 2 * hk) * d or cos_sin.shape[-1] != d:
         raise RuntimeError("block_append: qkv [T, (Hq + 2 Hk) D], cos_sin [positions, D]")
+    if fmt != K.FMT_BF16 and not (k_scale > 0 and v_scale > 0):
+        raise RuntimeError("the pool's scales must be positive")
     x = qkv[:, : (hq + 2 * hk) * d].float().unflatten(1, (hq + 2 * hk, d))
     ok = (pos >= 0) & (pos < cos_sin.shape[0])
     at = torch.where(ok, pos, torch.zeros_like(pos))
@@ -102,6 +104,8 @@ def block_summarize(pool: torch.Tensor, pages: torch.Tensor, codes: torch.Tensor
         ext().block_summarize(pool, pages, codes, scale, fmt, k_scale, hk, d)
         return
     _check_pool(pool, codes, scale, fmt, hk, d)
+    if fmt != K.FMT_BF16 and not k_scale > 0:
+        raise RuntimeError("the pool's scale must be positive")
     for p in pages.tolist():
         if not 0 <= p < pool.shape[0]:
             continue
@@ -212,7 +216,7 @@ def block_decode(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
         lse = torch.empty(q.shape[0], q.shape[1], dtype=torch.float32)
     _check_groups(q, page_table, kv_len, n_q, hk)
     _check_pool(pool, None, None, fmt, hk, q.shape[2])
-    if not (sm_scale > 0 and k_scale > 0):
+    if not (sm_scale > 0 and (fmt == K.FMT_BF16 or k_scale > 0)):
         raise RuntimeError("the softmax scale and the pool's key scale must be positive")
     if tuple(blocks.shape[:2]) != (kv_len.shape[0], hk) or not 1 <= blocks.shape[2] <= MAX_LIST:
         raise RuntimeError(f"blocks [B, Hk, 1 .. {MAX_LIST}]")

@@ -136,9 +136,18 @@ def test_refusals():
         S.block_decode(q[-1:], pool, table, kv, torch.zeros(1, 2, 4, dtype=torch.int32), 1, 2, 1, 0.1)
     with pytest.raises(RuntimeError):
         S.block_summarize(pool, torch.tensor([1]), codes[:1], sc, 0, 2, 128)
-    for kw in (dict(sm_scale=0.0), dict(sm_scale=-0.1), dict(sm_scale=0.1, k_scale=0.0)):
+    for kw in (dict(sm_scale=0.0), dict(sm_scale=-0.1), dict(sm_scale=float("nan"))):
         with pytest.raises(RuntimeError):
             S.block_decode(q[-1:], pool, table, kv, torch.zeros(1, 2, 4, dtype=torch.int32), 1, 2, 0, **kw)
+    q, pool, table, codes, sc, *_ = session(K.FMT_FP8, 70)
+    with pytest.raises(RuntimeError):
+        S.block_decode(q[-1:], pool, table, kv, torch.zeros(1, 2, 4, dtype=torch.int32), 1, 2, 1, 0.1, k_scale=0.0)
+    with pytest.raises(RuntimeError):
+        S.block_summarize(pool, torch.tensor([1]), codes, sc, 1, 2, 128, k_scale=-1.0)
+    with pytest.raises(RuntimeError):
+        S.block_append(torch.zeros(1, 8 * 128, dtype=torch.bfloat16), None, None, rope_table(4, 128, 1e4),
+                       torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), pool, codes, sc, 1, 4, 2,
+                       128, 1e-6, True, 1.0, 0.0)
 
 
 # ------------------------------------------------------------------------------------------------ engine

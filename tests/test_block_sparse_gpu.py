@@ -233,6 +233,16 @@ def test_select_of_long_requests_strided_q(cuda):
         assert torch.equal(got[0].cpu(), want[0])
 
 
+def test_select_at_the_widest_table(cuda):
+    """3.1 million tokens: every key of the selection fits the first CTA's shared memory; one page more is refused."""
+    d, hk, hq = 128, 1, 2
+    codes, sc = rand_bounds(5000, hk, d, 17, 12.0)
+    table = torch.randint(0, 5000, (1, S.MAX_PAGES), dtype=torch.int32)
+    q = torch.randn(1, hq, d).to(torch.bfloat16)
+    for n in (S.MAX_PAGES * 64, S.MAX_PAGES * 64 - 130, S.MAX_PAGES * 64 + 1000):
+        run_select(cuda, q, codes, sc, table, torch.tensor([n], dtype=torch.int32), 1, hk, 500)
+
+
 # ------------------------------------------------------------------------------------------------ attend
 def check_attend(got, lse, q, pool, table, kv, blocks, n_q, hk, fmt, sm, req=None):
     """Element bounds: P is rounded to 16 bits (relative 2^-9 bf16, 2^-12 f16, at least as fine) and the output to
@@ -523,6 +533,17 @@ def test_refusals(cuda):
             app(**k)
     with pytest.raises(RuntimeError):
         S.block_summarize(pool, i2.long(), codes, sc, 0, hk, d)
+    for k in (dict(sm_scale=0.0), dict(sm_scale=-1.0), dict(sm_scale=math.nan)):
+        with pytest.raises(RuntimeError):
+            ok(**k)
+    q8, pool8, *_ = attend_case(cuda, d, hq, hk, 1, K.FMT_FP8, [200, 100], 4, 1)
+    codes8, sc8 = S.alloc_bounds(pool8.shape[0], hk, d, cuda)
+    with pytest.raises(RuntimeError):
+        ok(pool=pool8, fmt=K.FMT_FP8, k_scale=0.0)
+    with pytest.raises(RuntimeError):
+        app(pool=pool8, codes=codes8, scale=sc8, fmt=K.FMT_FP8, v_scale=-1.0)
+    with pytest.raises(RuntimeError):
+        S.block_summarize(pool8, i2, codes8, sc8, K.FMT_FP8, hk, d, k_scale=0.0)
 
 
 # ------------------------------------------------------------------------------------------------ engine
