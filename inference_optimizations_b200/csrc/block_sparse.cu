@@ -28,12 +28,20 @@ __device__ __forceinline__ int code8(float v, float inv) {
 }
 
 // ------------------------------------------------------------------------------------------ head vectors
-// A warp holds one head vector of D values: lane l owns D / 64 consecutive values of each half, so both members of
-// every rotated pair (i, i + D / 2) are in one thread.  Values go in pairs: one instruction handles two fp32.
+// D / 16 lanes hold one head vector, so a warp holds 4, 2 or 1 of them (D = 128, 256, 512): lane l of a vector owns 8
+// consecutive values of each half (16-byte accesses), so both members of every rotated pair (i, i + D / 2) are in one
+// thread.  Values go in pairs: one instruction handles two fp32.
 template <int D>
 struct Lane {
-  static constexpr int H2 = D / 64;     // values of one half
+  static constexpr int H2 = 8;          // values of one half
   static constexpr int P = H2 / 2;      // pairs of one half
+  static constexpr int N = D / 16;      // lanes of a vector
+  static constexpr int PER_WARP = 32 / N;
+  static __device__ __forceinline__ int in_vector() { return lane_id() % N; }
+  static __device__ __forceinline__ int vector() { return lane_id() / N; }
+  static __device__ __forceinline__ uint32_t mask() {      // the lanes of this lane's vector
+    return N == 32 ? 0xffffffffu : ((1u << (N & 31)) - 1u) << (vector() * N);
+  }
 };
 
 template <int BYTES>
@@ -169,7 +177,7 @@ __device__ __forceinline__ Head<D> store_row(uint8_t* part, int off, int lane, f
         amax = fmaxf(amax, fmaxf(fabsf(y[j].x), fabsf(y[j].y)));
       }
 #pragma unroll
-      for (int o = 1; o < LPB; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      for (int o = 1; o < LPB; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(Lane<D>::mask(), amax, o));
       const uint8_t s8 = nvfp4_block_scale(amax);
       const float sf = e4m3_to_float(s8), inv_sf = 1.f / sf;
       if ((lane % LPB) == 0) part[kPage * (D / 2) + off * (D / 16) + e0 / 16] = s8;
@@ -250,7 +258,10 @@ __device__ __forceinline__ void norm_rope(const Head<D>& raw, float2 (&x)[2 * La
     float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < 2 * P; ++j) ss = fma2(x[j], x[j], ss);
-    const float inv = rsqrtf(warp_sum(ss.x + ss.y) / D + eps);
+    float sum = ss.x + ss.y;
+#pragma unroll
+    for (int o = 1; o < Lane<D>::N; o <<= 1) sum += __shfl_xor_sync(Lane<D>::mask(), sum, o);
+    const float inv = rsqrtf(sum / D + eps);
 #pragma unroll
     for (int j = 0; j < 2 * P; ++j) x[j] = mul2(mul2(x[j], make_float2(inv, inv)), gain[j]);
   }
@@ -312,9 +323,17 @@ __device__ void finish_bound(const Bound<D, FMT>& bd, float unit, int8_t* codes,
   for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-      const int d = hh * (D / 4) + lane * P + j;
-      sb[0][warp][d] = bd.lo[hh * P + j];
-      sb[1][warp][d] = bd.hi[hh * P + j];
+      uint32_t lo = bd.lo[hh * P + j], hi = bd.hi[hh * P + j];
+#pragma unroll
+      for (int o = Lane<D>::N; o < 32; o <<= 1) {          // the warp's vectors
+        lo = Bound<D, FMT>::low(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = Bound<D, FMT>::high(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      const int d = hh * (D / 4) + Lane<D>::in_vector() * P + j;
+      if (Lane<D>::vector() == 0) {
+        sb[0][warp][d] = lo;
+        sb[1][warp][d] = hi;
+      }
     }
   __syncthreads();
   constexpr int PER = D / 2 >= NT ? D / 2 / NT : 1;       // pairs of a thread (threads past D / 2 idle)
@@ -382,49 +401,51 @@ __device__ __forceinline__ int row_slot(const BlockAppendArgs& a, int t) {
 }
 
 template <int D, int FMT>
-__global__ void __launch_bounds__(kWarps * 32, D == 512 ? 5 : 6) block_append_kernel(const BlockAppendArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, 5) block_append_kernel(const BlockAppendArgs a) {
   __shared__ uint32_t red[2][kWarps][D / 2];
-  const int warp = warp_id(), lane = lane_id();
+  constexpr int NV = Lane<D>::PER_WARP;
+  const int warp = warp_id(), lane = lane_id(), ln = Lane<D>::in_vector(), vec = Lane<D>::vector();
   const int t0 = blockIdx.y * a.slab, t1 = min(a.T, t0 + a.slab);
   const __nv_bfloat16* qkv = reinterpret_cast<const __nv_bfloat16*>(a.qkv);
   constexpr int part = FMT == kKvBf16 ? kPage * 2 * D : FMT == kKvFp8 ? kPage * D : kPage * (D / 2 + D / 16);
   float2 x[2 * Lane<D>::P], gain[2 * Lane<D>::P];
   Angles<D> an;
   if (static_cast<int>(blockIdx.x) >= a.Hk) {
-    // a warp per row where there are rows for it, else a warp per head
+    // a warp per row where there are rows for it, else a warp per NV heads
     const int first = (blockIdx.x - a.Hk) * a.heads;
     const int vend = min(first + a.heads, a.Hq + a.Hk);
-    const int v0 = first + (a.slab == 1 ? warp : 0), vstep = a.slab == 1 ? kWarps : 1;
+    const int v0 = first + (a.slab == 1 ? warp * NV : 0), vstep = a.slab == 1 ? kWarps * NV : NV;
     if (v0 >= vend) return;
-    if (a.q_norm && v0 < a.Hq) load_gain<D>(a.q_norm, a.plus_one, lane, gain);
+    if (a.q_norm && v0 < a.Hq) load_gain<D>(a.q_norm, a.plus_one, ln, gain);
     const float inv = FMT == kKvBf16 ? 1.f : 1.f / a.v_scale;
     for (int t = t0 + (a.slab == 1 ? 0 : warp); t < t1; t += (a.slab == 1 ? 1 : kWarps)) {
       const __nv_bfloat16* src = qkv + static_cast<size_t>(t) * a.qkv_stride;
-      auto head = [&](int v) { return fetch<D>(src + static_cast<size_t>(v < a.Hq ? v : v + a.Hk) * D, lane); };
-      Head<D> next = head(v0), next2{};
-      if (v0 + vstep < vend) next2 = head(v0 + vstep);
+      auto head = [&](int v) {
+        return v < vend ? fetch<D>(src + static_cast<size_t>(v < a.Hq ? v : v + a.Hk) * D, ln) : Head<D>{};
+      };
+      Head<D> next = head(v0 + vec), next2 = head(v0 + vstep + vec);
       const int p = a.pos[t], s = row_slot(a, t);
       const bool ok = p >= 0 && p < a.max_pos;
-      if (ok && v0 < a.Hq) an.load(a.cos_sin + static_cast<size_t>(p) * D, lane);
+      if (ok && v0 < a.Hq) an.load(a.cos_sin + static_cast<size_t>(p) * D, ln);
       __nv_bfloat16* qrow = reinterpret_cast<__nv_bfloat16*>(a.q_out) + static_cast<size_t>(t) * a.Hq * D;
       uint8_t* vrow = a.pool + static_cast<size_t>(s < 0 ? 0 : s / kPage) * a.Hk * (2 * part) + part;
-      for (int v = v0; v < vend; v += vstep) {
+      for (int vb = v0; vb < vend; vb += vstep) {
+        const int v = vb + vec;
         const Head<D> raw = next;
-        const int vn = v + 2 * vstep;
         next = next2;
-        if (vn < vend) next2 = head(vn);
-        if (v < a.Hq) {
+        next2 = head(v + 2 * vstep);
+        if (v < a.Hq && v < vend) {
           Head<D> o{};
           if (ok) {
             norm_rope<D>(raw, x, gain, a.q_norm != nullptr, a.eps, an);
 #pragma unroll
             for (int j = 0; j < 2 * Lane<D>::P; ++j) o.w[j] = to_bf2(x[j]);
           }
-          store_head<D>(qrow + static_cast<size_t>(v) * D, lane, o);
-        } else if (s >= 0) {
+          store_head<D>(qrow + static_cast<size_t>(v) * D, ln, o);
+        } else if (v < vend && s >= 0) {
 #pragma unroll
           for (int j = 0; j < 2 * Lane<D>::P; ++j) x[j] = bf2(raw.w[j]);
-          store_row<D, FMT>(vrow + static_cast<size_t>(v - a.Hq) * (2 * part), s % kPage, lane, inv, x);
+          store_row<D, FMT>(vrow + static_cast<size_t>(v - a.Hq) * (2 * part), s % kPage, ln, inv, x);
         }
       }
     }
@@ -432,7 +453,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 512 ? 5 : 6) block_append_ke
   }
   const int h = blockIdx.x;
   const float unit = FMT == kKvBf16 ? 1.f : a.k_scale, inv = 1.f / unit;
-  if (a.k_norm) load_gain<D>(a.k_norm, a.plus_one, lane, gain);
+  if (a.k_norm) load_gain<D>(a.k_norm, a.plus_one, ln, gain);
   // rows of the slab (at most 32) that begin a run: every lane looks at one
   const int ts = t0 + lane;
   const int mine = ts < t1 ? row_slot(a, ts) : -1;
@@ -453,18 +474,20 @@ __global__ void __launch_bounds__(kWarps * 32, D == 512 ? 5 : 6) block_append_ke
     Bound<D, FMT> bd;
     bd.reset();
     const __nv_bfloat16* src = qkv + static_cast<size_t>(t) * a.qkv_stride + static_cast<size_t>(a.Hq + h) * D;
-    Head<D> next;
-    if (warp < n) next = fetch<D>(src + warp * a.qkv_stride, lane);
-    for (int i = warp; i < n; i += kWarps) {
-      an.load(a.cos_sin + static_cast<size_t>(a.pos[t + i]) * D, lane);
+    Head<D> next{};
+    if (warp * NV + vec < n) next = fetch<D>(src + (warp * NV + vec) * a.qkv_stride, ln);
+    for (int i = warp * NV + vec; i < n; i += kWarps * NV) {
+      an.load(a.cos_sin + static_cast<size_t>(a.pos[t + i]) * D, ln);
       const Head<D> raw = next;
-      if (i + kWarps < n) next = fetch<D>(src + (i + kWarps) * a.qkv_stride, lane);
+      if (i + kWarps * NV < n) next = fetch<D>(src + (i + kWarps * NV) * a.qkv_stride, ln);
       norm_rope<D>(raw, x, gain, a.k_norm != nullptr, a.eps, an);
-      bd.add(store_row<D, FMT>(base, off + i, lane, inv, x));
+      bd.add(store_row<D, FMT>(base, off + i, ln, inv, x));
     }
+    __syncwarp();
     if (!last) continue;
 #pragma unroll 4
-    for (int i = warp; i < off; i += kWarps) bd.add(load_row<D, FMT>(base, i, lane));
+    for (int i = warp * NV + vec; i < off; i += kWarps * NV) bd.add(load_row<D, FMT>(base, i, ln));
+    __syncwarp();
     const size_t ph = static_cast<size_t>(page) * a.Hk + h;
     finish_bound<D, FMT>(bd, unit, a.codes + ph * 2 * D, reinterpret_cast<__nv_bfloat16*>(a.scale) + ph, red);
   }
@@ -481,7 +504,8 @@ __global__ void __launch_bounds__(kWarps * 32) block_summarize_kernel(const Bloc
   Bound<D, FMT> bd;
   bd.reset();
 #pragma unroll 4
-  for (int i = warp_id(); i < kPage; i += kWarps) bd.add(load_row<D, FMT>(base, i, lane_id()));
+  for (int i = warp_id() * Lane<D>::PER_WARP + Lane<D>::vector(); i < kPage; i += kWarps * Lane<D>::PER_WARP)
+    bd.add(load_row<D, FMT>(base, i, Lane<D>::in_vector()));
   const size_t ph = static_cast<size_t>(page) * a.Hk + h;
   finish_bound<D, FMT>(bd, FMT == kKvBf16 ? 1.f : a.k_scale, a.codes + ph * 2 * D,
                        reinterpret_cast<__nv_bfloat16*>(a.scale) + ph, red);
@@ -835,7 +859,7 @@ cudaError_t block_append(const BlockAppendArgs& a_, cudaStream_t s) {
   if (a.T > 65535 * 16) return cudaErrorInvalidValue;      // the grid's second dimension
   // A decode step (few rows, each its own page) wants a CTA per row; a prefill wants fewer, longer CTAs.
   a.slab = a.T <= 256 ? 1 : 16;
-  a.heads = 4;
+  a.heads = 4 * (512 / a.D);
   IOB_BY_D_FMT(append_launch, a, s)
 }
 
