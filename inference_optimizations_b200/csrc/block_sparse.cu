@@ -859,7 +859,9 @@ cudaError_t block_append(const BlockAppendArgs& a_, cudaStream_t s) {
   if (a.T > 65535 * 16) return cudaErrorInvalidValue;      // the grid's second dimension
   // A decode step (few rows, each its own page) wants a CTA per row; a prefill wants fewer, longer CTAs.
   a.slab = a.T <= 256 ? 1 : 16;
-  a.heads = 4 * (512 / a.D);
+  // Heads of a q / v CTA: one per vector of its warps for a step; in a prefill a warp walks through 4 (D = 512) or through
+  // 2 vectors' worth, which shares the angles and keeps enough CTAs (7 x 219 rows of D = 256: 26.1 us, twice as many 28.0).
+  a.heads = a.slab == 1 ? 4 * (512 / a.D) : a.D == 512 ? 4 : 2 * (512 / a.D);
   IOB_BY_D_FMT(append_launch, a, s)
 }
 
