@@ -819,16 +819,18 @@ cudaError_t select_launch_v(const BlockSelectArgs& a, int cs, cudaStream_t s) {
 template <int D, bool R8>
 cudaError_t select_launch_r(const BlockSelectArgs& a, cudaStream_t s) {
   // Thousands of lists (a prefill chunk): small CTAs, many on an SM, so that one's selection runs under another's
-  // scores.  Enough to fill the SMs: the same with larger CTAs.  Few: the candidates of a list are split over a
-  // cluster until the SMs have two CTAs each, as long as a CTA keeps 64 pages, with 16 loads in flight per thread.
-  // (The page table's width bounds the candidates.)  Measured with each of the three forms, many / some / few: 512
-  // groups x 8 heads x 544 pages of D = 128: 84 / 98 / 141 us; 32 x 16 x 512 pages of D = 512: 50 / 38 / 45 us;
-  // 1 x 8 x 3200 pages of D = 128: 56 / 32 / 10 us.
+  // scores.  Enough to fill the SMs twice over: the same with larger CTAs; up to twice: with twice as large ones, whose
+  // selection is shorter.  Few: the candidates of a list are split over a cluster until the SMs have two CTAs each, as
+  // long as a CTA keeps 64 pages, with 16 loads in flight per thread.  (The page table's width bounds the candidates.)
+  // Measured, many / some / few: 512 groups x 8 heads x 544 pages of D = 128: 84 / 98 / 141 us; 32 x 16 x 512 pages of
+  // D = 512: 50 / 38 / 45 us; 1 x 8 x 3200 pages of D = 128: 56 / 32 / 10 us; some with 256 / 512 threads: 32 x 16 lists
+  // 38 / 42 us, 16 x 16 lists 28 / 23 us.
   const int units = a.B * a.Hk;
   const int var = units >= 148 * 8 ? 2 : units > 148 ? 1 : 0;
   int cs = 1;
   while (var == 0 && cs < 8 && units * cs * 2 <= 2 * 148 && a.pt_stride >= 128 * cs) cs *= 2;
   if (var == 2) return select_launch_v<D, R8, 128, 1, 8>(a, cs, s);
+  if (var == 1 && units <= 2 * 148) return select_launch_v<D, R8, 512, 1, 2>(a, cs, s);
   if (var == 1) return select_launch_v<D, R8, 256, 1, 4>(a, cs, s);
   return select_launch_v<D, R8, 256, 1024 / (2 * D), 2>(a, cs, s);
 }

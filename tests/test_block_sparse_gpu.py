@@ -233,6 +233,20 @@ def test_select_of_long_requests_strided_q(cuda):
         assert torch.equal(got[0].cpu(), want[0])
 
 
+@pytest.mark.parametrize("groups", [80, 200, 640])
+@pytest.mark.parametrize("d,hq,n_q", [(128, 4, 1), (256, 8, 3), (512, 6, 4)])
+def test_select_many_lists(cuda, groups, d, hq, n_q):
+    """160, 400 and 1280 lists: every form of the selection, 8 and 16 query rows."""
+    hk = 2
+    codes, sc = rand_bounds(150, hk, d, groups)
+    g = torch.Generator().manual_seed(groups)
+    table = torch.stack([torch.randperm(150, generator=g)[:70] for _ in range(9)]).to(torch.int32)
+    kv = torch.randint(0, 70 * 64 + 1, (groups,), generator=g).to(torch.int32)
+    req = torch.randint(0, 9, (groups,), generator=g).to(torch.int32)
+    q = torch.randn(groups * n_q, hq, d, generator=g).to(torch.bfloat16)
+    run_select(cuda, q, codes, sc, table, kv, n_q, hk, 11, req_idx=req)
+
+
 def test_select_at_the_widest_table(cuda):
     """3.1 million tokens: every key of the selection fits the first CTA's shared memory; one page more is refused."""
     d, hk, hq = 128, 1, 2
