@@ -18,8 +18,8 @@
 //
 // Bound by the listed pages' bytes over bf16 and E4M3 caches (16 x 16 lists of 32 pages of D = 512, bf16: 144 us, 6.7
 // TB/s; 64 x 8 lists of D = 128, E4M3: 49.5 us, 5.4 TB/s), by the conversions over FP4 caches (32 x 16 lists of 64 pages
-// of D = 512: 271 us, 4.2 TB/s), by launch and load latency for one user (8 lists of 32 pages of D = 128: 8.7 us), by the
-// path from L2 for a prefill's groups (512 x 8 lists of 32 pages, 4.3 GB, of a 35k-token request: 325 us).
+// of D = 512: 265 us, 4.3 TB/s), by launch and load latency for one user (8 lists of 32 pages of D = 128: 8.0 us), by the
+// path from L2 for a prefill's groups (512 x 8 lists of 32 pages, 4.3 GB, of a 35k-token request: 315 us).
 #include "common.cuh"
 #include "kernels.h"
 
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ __align__(8) uint64_t full[kWarps][C::NS];
   __shared__ float s_wm[kWarps][ROWS], s_wl[kWarps][ROWS], s_wn[kWarps][ROWS], s_m[ROWS], s_l[ROWS], s_n[ROWS],
-      s_qf[ROWS], s_f[8][ROWS];
+      s_qf[ROWS], s_f[8][ROWS], s_cl[8][ROWS], s_cn[8][ROWS];
   __shared__ int s_cnt, s_abort;
   int* s_blk = reinterpret_cast<int*>(sm + C::off_list);
   int* s_phys = s_blk + cap;
@@ -614,17 +614,26 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   // ---- join of the cluster: every CTA finishes its share of the R x D outputs
   if (csize > 1) cluster_sync_all();
   else __syncthreads();
-  const uint32_t am = smem_u32(s_m), al = smem_u32(s_l), an = smem_u32(s_n), ao = smem_u32(sm);
+  // (the CTAs' statistics are fetched by as many threads, the outputs' parts all before their sum: one remote latency
+  // each, not one per CTA)
+  const uint32_t ao = smem_u32(sm);
+  static_assert(8 * ROWS <= kThreads, "a thread per CTA and row");
+  if (tid < csize * ROWS) {
+    const int c = tid / ROWS, r = tid % ROWS;
+    s_f[c][r] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&s_m[r]), c)));
+    s_cl[c][r] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&s_l[r]), c)));
+    s_cn[c][r] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&s_n[r]), c)));
+  }
+  __syncthreads();
   if (tid < ROWS) {
-    float M = -INFINITY;
-    for (int c = 0; c < csize; ++c) M = fmaxf(M, __uint_as_float(ld_cluster_u32(mapa_shared(am + 4 * tid, c))));
+    float M = -INFINITY, L = 0.f, N = 0.f;
+    for (int c = 0; c < csize; ++c) M = fmaxf(M, s_f[c][tid]);
     const float ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f, N = 0.f;
     for (int c = 0; c < csize; ++c) {
-      const float f = ex2(__uint_as_float(ld_cluster_u32(mapa_shared(am + 4 * tid, c))) - ms);
+      const float f = ex2(s_f[c][tid] - ms);
       s_f[c][tid] = f;
-      L += f * __uint_as_float(ld_cluster_u32(mapa_shared(al + 4 * tid, c)));
-      N += f * __uint_as_float(ld_cluster_u32(mapa_shared(an + 4 * tid, c)));
+      L += f * s_cl[c][tid];
+      N += f * s_cn[c][tid];
     }
     const float inv = L == 0.f ? 0.f : (C::BF ? 1.f : a.v_scale) / N;
     for (int c = 0; c < csize; ++c) s_f[c][tid] *= inv;
@@ -636,15 +645,19 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out);
   for (int i = rank * kThreads + tid; i < R * (C::D / 4); i += csize * kThreads) {
     const int row = i / (C::D / 4), d = 4 * (i % (C::D / 4));
+    float4 v[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < csize) v[c] = ld_cluster_f4(mapa_shared(ao + 4 * (row * C::DP + d), c));
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < csize; ++c) {
-      const float f = s_f[c][row];
-      const float4 v = ld_cluster_f4(mapa_shared(ao + 4 * (row * C::DP + d), c));
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const float f = c < csize ? s_f[c][row] : 0.f;
       if (f != 0.f) {
-        o.x += f * v.x;
-        o.y += f * v.y;
-        o.z += f * v.z;
-        o.w += f * v.w;
+        o.x += f * v[c].x;
+        o.y += f * v[c].y;
+        o.z += f * v[c].z;
+        o.w += f * v[c].w;
       }
     }
     uint2 raw;
