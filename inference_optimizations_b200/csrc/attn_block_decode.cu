@@ -18,7 +18,7 @@
 //
 // Bound by the listed pages' bytes over bf16 and E4M3 caches (16 x 16 lists of 32 pages of D = 512, bf16: 144 us, 6.7
 // TB/s; 64 x 8 lists of D = 128, E4M3: 49.5 us, 5.4 TB/s), by the conversions over FP4 caches (32 x 16 lists of 64 pages
-// of D = 512: 265 us, 4.3 TB/s), by launch and load latency for one user (8 lists of 32 pages of D = 128: 8.0 us), by the
+// of D = 512: 249 us, 4.6 TB/s), by launch and load latency for one user (8 lists of 32 pages of D = 128: 8.0 us), by the
 // path from L2 for a prefill's groups (512 x 8 lists of 32 pages, 4.3 GB, of a 35k-token request: 315 us).
 #include "common.cuh"
 #include "kernels.h"
@@ -36,10 +36,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 // of the rounded weights (a row of ones beside V), so that the rounding of a weight that dominates its row cancels; the
 // log-sum-exp takes the sum of the unrounded ones.
 constexpr float kLag = 8.f;
+// Where P also takes a block scale (2^-9 .. 448) in f16: 2^kUp in front keeps small products out of the subnormals, and
+// with the shorter lag the largest is 2^6 x 448.
+constexpr float kLagTwice = 3.f, kUp = 3.f;
 
-template <int D_, int FMT_, int NR_>
+template <int D_, int FMT_, int NR_, bool TWICE_ = false>
 struct Cfg {
   static constexpr int D = D_, FMT = FMT_, NR = NR_;       // NR: groups of 8 query rows
+  // Up to 4 rows over an FP4 cache stand in the 8 columns twice: a lane's rows of V^T lie in one of a 32-value chunk's
+  // two scale blocks, columns 0 .. 3 carry P times the first block's scales, 4 .. 7 times the second's, and each
+  // half of O^T is taken from the columns that fit.  V's codes are then used as they are: one product with the
+  // scales per chunk and 8 tokens instead of four (D = 512, 32 x 16 lists of 64 pages: 249 against 265 us).
+  static constexpr bool TWICE = TWICE_;
+  static_assert(!TWICE || (FMT == kKvNvfp4 && NR == 1), "two scale blocks of a chunk");
   static constexpr bool BF = FMT == kKvBf16;
   static constexpr int RB = BF ? 2 * D : FMT == kKvFp8 ? D : D / 2;       // bytes of a row
   static constexpr int SC = FMT == kKvNvfp4 ? D / 16 : 0;                 // block scale bytes of a row
@@ -207,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ __align__(8) uint64_t full[kWarps][C::NS];
   __shared__ float s_wm[kWarps][ROWS], s_wl[kWarps][ROWS], s_wn[kWarps][ROWS], s_m[ROWS], s_l[ROWS], s_n[ROWS],
-      s_qf[ROWS], s_f[8][ROWS], s_cl[8][ROWS], s_cn[8][ROWS];
+      s_qf[ROWS], s_f[8][ROWS];
   __shared__ int s_cnt, s_abort;
   int* s_blk = reinterpret_cast<int*>(sm + C::off_list);
   int* s_phys = s_blk + cap;
@@ -219,6 +228,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   const int prow = a.req_idx ? a.req_idx[b] : b;
   const int len = (prow < 0 || prow >= a.rows) ? 0 : min(a.kv_len[b], a.pt_stride * kPage);
   const int q0 = len - a.n_q;                    // position of the group's first token (may be negative)
+  auto row_of = [](int col) { return C::TWICE ? col & 3 : col; };      // query row of a column
   auto q_row = [&](int r) -> const __nv_bfloat16* {
     if (r >= R) return nullptr;
     return reinterpret_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(b * a.n_q + (r0 + r) / G) * a.q_stride +
@@ -272,8 +282,8 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   uint2* s_q = reinterpret_cast<uint2*>(sm + C::off_q) + lane;      // [KK][NR][32]
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
-    const __nv_bfloat16* q = q_row(8 * n + g);
-    const float f = C::BF ? 1.f : 1.f / s_qf[8 * n + g];
+    const __nv_bfloat16* q = q_row(row_of(8 * n + g));
+    const float f = C::BF ? 1.f : 1.f / s_qf[row_of(8 * n + g)];
 #pragma unroll
     for (int kk = 0; kk < C::KK; ++kk) {
       if (C::QSM && kk % kWarps != warp) continue;                  // shared: each warp prepares its part
@@ -305,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   float scale[2 * NR], m[2 * NR], l[2 * NR];
 #pragma unroll
   for (int i = 0; i < 2 * NR; ++i) {
-    const int r = 8 * (i >> 1) + 2 * j4 + (i & 1);
+    const int r = row_of(8 * (i >> 1) + 2 * j4 + (i & 1));
     scale[i] = a.sm_scale * kLog2e * (C::BF ? 1.f : a.k_scale * s_qf[r]);
     m[i] = -INFINITY;
     l[i] = 0.f;
@@ -423,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
       for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int vis = min(len, q0 + (r0 + 8 * n + 2 * j4 + e) / G + 1) - base - g;
+          const int vis = min(len, q0 + (r0 + row_of(8 * n + 2 * j4 + e)) / G + 1) - base - g;
 #pragma unroll
           for (int u = 0; u < C::SUB; ++u) {
             if (16 * u >= vis) s[u][n][e] = -INFINITY;
@@ -441,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
       mt[i] = x;
-      over |= (x - m[i]) * scale[i] > kLag;      // (m = -inf: any finite score; a score of -inf never)
+      over |= (x - m[i]) * scale[i] > (C::TWICE ? kLagTwice : kLag);      // (m = -inf: any finite score; a score of -inf never)
     }
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -461,8 +471,9 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
     uint32_t p[C::SUB][NR][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      const float c0 = m[2 * n] == -INFINITY ? 0.f : -m[2 * n] * scale[2 * n];
-      const float c1 = m[2 * n + 1] == -INFINITY ? 0.f : -m[2 * n + 1] * scale[2 * n + 1];
+      constexpr float up = C::TWICE ? kUp : 0.f;
+      const float c0 = m[2 * n] == -INFINITY ? 0.f : up - m[2 * n] * scale[2 * n];
+      const float c1 = m[2 * n + 1] == -INFINITY ? 0.f : up - m[2 * n + 1] * scale[2 * n + 1];
 #pragma unroll
       for (int u = 0; u < C::SUB; ++u) {
 #pragma unroll
@@ -528,22 +539,31 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
                                   prmt(sv[1][0], sv[1][1], 0x6240u + (lane >> 4) * 0x1111u)};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {          // a chunk of 32 values: 4 g + {0 .. 3}
-            uint32_t v[2][4];
+            uint32_t v[2][4], ps[2];
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
               const uint32_t s2 = e4m3x2(e ? pr[o] >> 16 : pr[o]);
               uint32_t w[4];                     // (0, 1) (2, 3) of token 2 j4, then of 2 j4 + 1
               e2m1x8(r[2 * o + e], w);
-              v[o][0] = hmul2_u32(prmt(w[0], w[2], 0x5410u), s2);
-              v[o][1] = hmul2_u32(prmt(w[0], w[2], 0x7632u), s2);
-              v[o][2] = hmul2_u32(prmt(w[1], w[3], 0x5410u), s2);
-              v[o][3] = hmul2_u32(prmt(w[1], w[3], 0x7632u), s2);
+              v[o][0] = prmt(w[0], w[2], 0x5410u);
+              v[o][1] = prmt(w[0], w[2], 0x7632u);
+              v[o][2] = prmt(w[1], w[3], 0x5410u);
+              v[o][3] = prmt(w[1], w[3], 0x7632u);
+              if constexpr (C::TWICE) {
+                ps[o] = hmul2_u32(p[u][0][o], s2);         // (column g: block g / 4 of the chunk)
+              } else {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[o][x] = hmul2_u32(v[o][x], s2);
+              }
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
               const uint32_t f[4] = {v[0][2 * t], v[0][2 * t + 1], v[1][2 * t], v[1][2 * t + 1]};
 #pragma unroll
-              for (int n = 0; n < NR; ++n) mma<false>(acc[4 * i + 2 * e + t][n], f, p[u][n]);
+              for (int n = 0; n < NR; ++n) {
+                if constexpr (C::TWICE) mma<false>(acc[4 * i + 2 * e + t][n], f, ps);
+                else mma<false>(acc[4 * i + 2 * e + t][n], f, p[u][n]);
+              }
             }
           }
         }
@@ -559,13 +579,13 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   for (int i = 0; i < 2 * NR; ++i) {
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
-    const int r = 8 * (i >> 1) + 2 * j4 + (i & 1);
+    const int r = row_of(8 * (i >> 1) + 2 * j4 + (i & 1));
     if (g == 0) {
-      s_wm[warp][r] = m[i] * scale[i];
+      s_wm[warp][r] = m[i] * scale[i] - (C::TWICE ? kUp : 0.f);
       s_wl[warp][r] = s_abort ? NAN : l[i];
       s_wn[warp][r] = s_abort ? NAN : C::BF ? accn[i >> 1][i & 1] : l[i];
     }
-    if (r < R) {
+    if (r < R && (!C::TWICE || (g >> 2) == (j4 >> 1))) {
 #pragma unroll
       for (int t = 0; t < C::MT; ++t) {
         int d, dn;                               // values of rows g, g + 8 of the tile
@@ -617,7 +637,9 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   // (the CTAs' statistics are fetched by as many threads, the outputs' parts all before their sum: one remote latency
   // each, not one per CTA)
   const uint32_t ao = smem_u32(sm);
-  static_assert(8 * ROWS <= kThreads, "a thread per CTA and row");
+  static_assert(8 * ROWS <= kThreads && 16 * ROWS * 4 <= C::RING, "a thread per CTA and row");
+  float(*s_cl)[ROWS] = reinterpret_cast<float(*)[ROWS]>(sm + C::RING);      // (the second warp's ring is free by now)
+  float(*s_cn)[ROWS] = s_cl + 8;
   if (tid < csize * ROWS) {
     const int c = tid / ROWS, r = tid % ROWS;
     s_f[c][r] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&s_m[r]), c)));
@@ -669,9 +691,9 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   if (csize > 1) cluster_sync_all();             // a CTA's partial results are read until here
 }
 
-template <int D, int FMT, int NR>
+template <int D, int FMT, int NR, bool TWICE = false>
 cudaError_t launch_r(const BlockDecodeArgs& a, int rgroups, cudaStream_t s) {
-  using C = Cfg<D, FMT, NR>;
+  using C = Cfg<D, FMT, NR, TWICE>;
   // Few lists: each is split over a cluster, as far as the SMs have room for all its CTAs at once and a CTA keeps two
   // pages.
   const int units = a.B * a.Hk * rgroups;
@@ -699,7 +721,11 @@ template <int D, int FMT>
 cudaError_t launch(const BlockDecodeArgs& a, cudaStream_t s) {
   // Up to 8 query rows: one column group.  More: two, or for D = 512, where a warp has no registers for two, two
   // clusters that read the same pages.
-  if (a.n_q * (a.Hq / a.Hk) <= 8) return launch_r<D, FMT, 1>(a, 1, s);
+  const int rows = a.n_q * (a.Hq / a.Hk);
+  if constexpr (FMT == kKvNvfp4) {
+    if (rows <= 4) return launch_r<D, FMT, 1, true>(a, 1, s);
+  }
+  if (rows <= 8) return launch_r<D, FMT, 1>(a, 1, s);
   if constexpr (D == 512) return launch_r<D, FMT, 1>(a, 2, s);
   else return launch_r<D, FMT, 2>(a, 1, s);
 }
