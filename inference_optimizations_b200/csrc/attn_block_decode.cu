@@ -18,7 +18,7 @@
 //
 // Bound by the listed pages' bytes over bf16 and E4M3 caches (16 x 16 lists of 32 pages of D = 512, bf16: 144 us, 6.7
 // TB/s; 64 x 8 lists of D = 128, E4M3: 49.5 us, 5.4 TB/s), by the conversions over FP4 caches (32 x 16 lists of 64 pages
-// of D = 512: 249 us, 4.6 TB/s), by launch and load latency for one user (8 lists of 32 pages of D = 128: 8.0 us), by the
+// of D = 512: 266 us, 4.3 TB/s), by launch and load latency for one user (8 lists of 32 pages of D = 128: 8.0 us), by the
 // path from L2 for a prefill's groups (512 x 8 lists of 32 pages, 4.3 GB, of a 35k-token request: 315 us).
 #include "common.cuh"
 #include "kernels.h"
@@ -30,25 +30,20 @@ constexpr int kPage = 64;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
-// The running maximum may lag behind the true one by this much in the base-2 exponentials: floating point keeps its
-// relative precision (P <= 2^8 in f16 as well), and the output is hardly ever rescaled after the first tiles.  P is
-// rounded for the second product, to 11 bits (f16) or, over a bf16 cache, to 8: there the output is divided by the sum
-// of the rounded weights (a row of ones beside V), so that the rounding of a weight that dominates its row cancels; the
-// log-sum-exp takes the sum of the unrounded ones.
-constexpr float kLag = 8.f;
-// Where P also takes a block scale (2^-9 .. 448) in f16: 2^kUp in front keeps small products out of the subnormals, and
-// with the shorter lag the largest is 2^6 x 448.
-constexpr float kLagTwice = 3.f, kUp = 3.f;
+// The running maximum may lag behind the true one by kLag in the base-2 exponentials: floating point keeps its relative
+// precision, and the output is hardly ever rescaled after the first tiles.  P is rounded for the second product, to 11
+// bits (f16) or, over a bf16 cache, to 8: there the output is divided by the sum of the rounded weights (a row of ones
+// beside V), so that the rounding of a weight that dominates its row cancels; the log-sum-exp takes the sum of the
+// unrounded ones.  f16 has 2^-14 as its smallest normal number, so P carries 2^kUp there (at most 2^15 with the lag):
+// weights down to 2^-26 of the largest keep their 11 bits, smaller ones are off by at most 2^-37 of it.
+template <bool BF>
+struct Weights {
+  static constexpr float kLag = BF ? 8.f : 3.f, kUp = BF ? 0.f : 12.f;
+};
 
-template <int D_, int FMT_, int NR_, bool TWICE_ = false>
+template <int D_, int FMT_, int NR_>
 struct Cfg {
   static constexpr int D = D_, FMT = FMT_, NR = NR_;       // NR: groups of 8 query rows
-  // Up to 4 rows over an FP4 cache stand in the 8 columns twice: a lane's rows of V^T lie in one of a 32-value chunk's
-  // two scale blocks, columns 0 .. 3 carry P times the first block's scales, 4 .. 7 times the second's, and each
-  // half of O^T is taken from the columns that fit.  V's codes are then used as they are: one product with the
-  // scales per chunk and 8 tokens instead of four (D = 512, 32 x 16 lists of 64 pages: 249 against 265 us).
-  static constexpr bool TWICE = TWICE_;
-  static_assert(!TWICE || (FMT == kKvNvfp4 && NR == 1), "two scale blocks of a chunk");
   static constexpr bool BF = FMT == kKvBf16;
   static constexpr int RB = BF ? 2 * D : FMT == kKvFp8 ? D : D / 2;       // bytes of a row
   static constexpr int SC = FMT == kKvNvfp4 ? D / 16 : 0;                 // block scale bytes of a row
@@ -212,6 +207,7 @@ __device__ __forceinline__ float row_pow2(const __nv_bfloat16* q) {
 template <class C>
 __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const BlockDecodeArgs a, const int csize,
                                                                         const int cap, const int rgroups) {
+  using W = Weights<C::BF>;
   constexpr int NR = C::NR, ROWS = 8 * NR;
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ __align__(8) uint64_t full[kWarps][C::NS];
@@ -228,7 +224,6 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   const int prow = a.req_idx ? a.req_idx[b] : b;
   const int len = (prow < 0 || prow >= a.rows) ? 0 : min(a.kv_len[b], a.pt_stride * kPage);
   const int q0 = len - a.n_q;                    // position of the group's first token (may be negative)
-  auto row_of = [](int col) { return C::TWICE ? col & 3 : col; };      // query row of a column
   auto q_row = [&](int r) -> const __nv_bfloat16* {
     if (r >= R) return nullptr;
     return reinterpret_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(b * a.n_q + (r0 + r) / G) * a.q_stride +
@@ -282,8 +277,8 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   uint2* s_q = reinterpret_cast<uint2*>(sm + C::off_q) + lane;      // [KK][NR][32]
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
-    const __nv_bfloat16* q = q_row(row_of(8 * n + g));
-    const float f = C::BF ? 1.f : 1.f / s_qf[row_of(8 * n + g)];
+    const __nv_bfloat16* q = q_row(8 * n + g);
+    const float f = C::BF ? 1.f : 1.f / s_qf[8 * n + g];
 #pragma unroll
     for (int kk = 0; kk < C::KK; ++kk) {
       if (C::QSM && kk % kWarps != warp) continue;                  // shared: each warp prepares its part
@@ -315,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   float scale[2 * NR], m[2 * NR], l[2 * NR];
 #pragma unroll
   for (int i = 0; i < 2 * NR; ++i) {
-    const int r = row_of(8 * (i >> 1) + 2 * j4 + (i & 1));
+    const int r = 8 * (i >> 1) + 2 * j4 + (i & 1);
     scale[i] = a.sm_scale * kLog2e * (C::BF ? 1.f : a.k_scale * s_qf[r]);
     m[i] = -INFINITY;
     l[i] = 0.f;
@@ -433,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
       for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int vis = min(len, q0 + (r0 + row_of(8 * n + 2 * j4 + e)) / G + 1) - base - g;
+          const int vis = min(len, q0 + (r0 + 8 * n + 2 * j4 + e) / G + 1) - base - g;
 #pragma unroll
           for (int u = 0; u < C::SUB; ++u) {
             if (16 * u >= vis) s[u][n][e] = -INFINITY;
@@ -451,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
       mt[i] = x;
-      over |= (x - m[i]) * scale[i] > (C::TWICE ? kLagTwice : kLag);      // (m = -inf: any finite score; a score of -inf never)
+      over |= (x - m[i]) * scale[i] > W::kLag;      // (m = -inf: any finite score; a score of -inf never)
     }
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -471,9 +466,8 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
     uint32_t p[C::SUB][NR][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      constexpr float up = C::TWICE ? kUp : 0.f;
-      const float c0 = m[2 * n] == -INFINITY ? 0.f : up - m[2 * n] * scale[2 * n];
-      const float c1 = m[2 * n + 1] == -INFINITY ? 0.f : up - m[2 * n + 1] * scale[2 * n + 1];
+      const float c0 = m[2 * n] == -INFINITY ? 0.f : W::kUp - m[2 * n] * scale[2 * n];
+      const float c1 = m[2 * n + 1] == -INFINITY ? 0.f : W::kUp - m[2 * n + 1] * scale[2 * n + 1];
 #pragma unroll
       for (int u = 0; u < C::SUB; ++u) {
 #pragma unroll
@@ -539,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
                                   prmt(sv[1][0], sv[1][1], 0x6240u + (lane >> 4) * 0x1111u)};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {          // a chunk of 32 values: 4 g + {0 .. 3}
-            uint32_t v[2][4], ps[2];
+            uint32_t v[2][4];
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
               const uint32_t s2 = e4m3x2(e ? pr[o] >> 16 : pr[o]);
@@ -549,21 +543,14 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
               v[o][1] = prmt(w[0], w[2], 0x7632u);
               v[o][2] = prmt(w[1], w[3], 0x5410u);
               v[o][3] = prmt(w[1], w[3], 0x7632u);
-              if constexpr (C::TWICE) {
-                ps[o] = hmul2_u32(p[u][0][o], s2);         // (column g: block g / 4 of the chunk)
-              } else {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) v[o][x] = hmul2_u32(v[o][x], s2);
-              }
+              for (int x = 0; x < 4; ++x) v[o][x] = hmul2_u32(v[o][x], s2);
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
               const uint32_t f[4] = {v[0][2 * t], v[0][2 * t + 1], v[1][2 * t], v[1][2 * t + 1]};
 #pragma unroll
-              for (int n = 0; n < NR; ++n) {
-                if constexpr (C::TWICE) mma<false>(acc[4 * i + 2 * e + t][n], f, ps);
-                else mma<false>(acc[4 * i + 2 * e + t][n], f, p[u][n]);
-              }
+              for (int n = 0; n < NR; ++n) mma<false>(acc[4 * i + 2 * e + t][n], f, p[u][n]);
             }
           }
         }
@@ -579,13 +566,13 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   for (int i = 0; i < 2 * NR; ++i) {
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
-    const int r = row_of(8 * (i >> 1) + 2 * j4 + (i & 1));
+    const int r = 8 * (i >> 1) + 2 * j4 + (i & 1);
     if (g == 0) {
-      s_wm[warp][r] = m[i] * scale[i] - (C::TWICE ? kUp : 0.f);
+      s_wm[warp][r] = m[i] * scale[i] - W::kUp;
       s_wl[warp][r] = s_abort ? NAN : l[i];
       s_wn[warp][r] = s_abort ? NAN : C::BF ? accn[i >> 1][i & 1] : l[i];
     }
-    if (r < R && (!C::TWICE || (g >> 2) == (j4 >> 1))) {
+    if (r < R) {
 #pragma unroll
       for (int t = 0; t < C::MT; ++t) {
         int d, dn;                               // values of rows g, g + 8 of the tile
@@ -691,9 +678,9 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   if (csize > 1) cluster_sync_all();             // a CTA's partial results are read until here
 }
 
-template <int D, int FMT, int NR, bool TWICE = false>
+template <int D, int FMT, int NR>
 cudaError_t launch_r(const BlockDecodeArgs& a, int rgroups, cudaStream_t s) {
-  using C = Cfg<D, FMT, NR, TWICE>;
+  using C = Cfg<D, FMT, NR>;
   // Few lists: each is split over a cluster, as far as the SMs have room for all its CTAs at once and a CTA keeps two
   // pages.
   const int units = a.B * a.Hk * rgroups;
@@ -722,9 +709,6 @@ cudaError_t launch(const BlockDecodeArgs& a, cudaStream_t s) {
   // Up to 8 query rows: one column group.  More: two, or for D = 512, where a warp has no registers for two, two
   // clusters that read the same pages.
   const int rows = a.n_q * (a.Hq / a.Hk);
-  if constexpr (FMT == kKvNvfp4) {
-    if (rows <= 4) return launch_r<D, FMT, 1, true>(a, 1, s);
-  }
   if (rows <= 8) return launch_r<D, FMT, 1>(a, 1, s);
   if constexpr (D == 512) return launch_r<D, FMT, 1>(a, 2, s);
   else return launch_r<D, FMT, 2>(a, 1, s);

@@ -1,0 +1,143 @@
+"""Accuracy of `block_decode` element by element against 64 bits, with a bound for each way the weights are held:
+requests with one dominating token, block scales from the smallest to the largest, queries that make scores large."""
+import functools
+import math
+
+import pytest
+import torch
+
+from inference_optimizations_b200.ops import block_sparse as S
+from inference_optimizations_b200.ops import kvcache as K
+
+pytestmark = pytest.mark.gpu
+
+FMTS = {"bf16": K.FMT_BF16, "fp8": K.FMT_FP8, "nvfp4": K.FMT_NVFP4}
+KS, VS = 0.75, 1.25
+# Relative rounding of a weight for the second product: 11 bits over 8-bit and 4-bit caches, 8 bits over bf16 ones.
+UNIT = {K.FMT_BF16: 2.0 ** -8, K.FMT_FP8: 2.0 ** -11, K.FMT_NVFP4: 2.0 ** -11}
+
+
+def part_abs(pool, fmt, d):
+    """The pool with |V|, and with |V| and |K|."""
+    out = []
+    for parts in (slice(1, 2), slice(0, 2)):
+        p = pool.clone()
+        if fmt == K.FMT_BF16:
+            p.view(torch.bfloat16)[:, :, parts].abs_()
+        elif fmt == K.FMT_FP8:
+            p[:, :, parts] &= 0x7F
+        else:
+            p[:, :, parts, :K.PAGE * d // 2] &= 0x77
+        out.append(p)
+    return out
+
+
+def check(out, lse, q, pool, table, kv, blocks, n_q, hk, fmt, sm):
+    """out: its own rounding to bf16 (2^-8), of each weight UNIT and twice the score's error, and where weights are f16
+    2^-37 of the largest for each of them (the last step of an f16 that carries 2^12).  Scores: an fp32 sum of D exact
+    products, at most D 2^-23 of the sum of their sizes, and the exponent's rounding, 2^-22 of the score each for its
+    scale and its difference.  lse: the scores' error, and 2^-20 of a sum of fp32 terms."""
+    d = q.shape[2]
+    c = [x.cpu() for x in (q, pool, table, kv, blocks)]
+
+    def ref(q_, pool_):
+        return S.block_decode_ref(q_, pool_, *c[2:], n_q, hk, fmt, sm, KS, VS, None, torch.float64)
+    want, wlse = ref(c[0], c[1])
+    va, ka = part_abs(c[1], fmt, d)
+    mag, _ = ref(c[0], va)
+    zero = torch.zeros_like(c[0])
+    total, count = ref(zero, va)
+    total = total * count.exp()[..., None]                            # sum of |v| over what a row sees
+    size = ref(c[0].abs(), ka)[1].clamp(min=0)                        # at least the largest sum of |q||k| sm
+    ds = (size * (d * 2.0 ** -23 + 2.0 ** -21) + 2.0 ** -20)[..., None]
+    tiny = 0.0 if fmt == K.FMT_BF16 else 2.0 ** -37
+    tol = want.abs() * 2.0 ** -8 + mag * (UNIT[fmt] + 2 * ds) + total * tiny + 1e-30
+    got = out.cpu().double()
+    off = (got - want).abs()
+    assert ((off <= tol) | (want.isnan() & got.isnan())).all(), f"{(off / tol).max()} of the bound"
+    near = (lse.cpu().double() - wlse).abs() <= ds[..., 0] + 2.0 ** -20 * (1 + wlse.abs())
+    assert (near | (lse.cpu() == wlse)).all()                         # (a row that sees nothing: -inf)
+
+
+@functools.lru_cache(maxsize=1)
+def dominated_pool(fmt, d, scale, seed):
+    g = torch.Generator().manual_seed(seed)
+    pages, n = 64, 4096
+    codes = torch.tensor([0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -1.0])
+    v = codes[torch.randint(0, 8, (n, 1, d), generator=g)]
+    v[:, :, ::16] = 6.0                                               # every block of 16 has the largest code
+    v = v * scale
+    v[17] = 0
+    k = torch.zeros(n, 1, d)
+    k[17, 0, 0] = 6.0
+    unit = (1.0, 1.0) if fmt == K.FMT_BF16 else (KS, VS)
+    pool = torch.zeros(pages + 1, 1, 2, K.part_bytes(fmt, d), dtype=torch.uint8)
+    table = (torch.randperm(pages, generator=g) + 1)[None].int()
+    at = torch.arange(n)
+    slot = (table[0, at // 64] * 64 + at % 64).int()
+    K.gqa_pool_write_ref(pool, slot, k * unit[0], v * unit[1], fmt, *unit)
+    return pool, table, unit
+
+
+def dominated(fmt, d, hq, gap, scale, seed):
+    """64 pages: token 17 has V = 0 and weight 1, every other token about 2^-gap; V in one scale, mostly positive (an
+    E4M3 cache cannot hold the largest scale's codes: the writer's NaN have to come out)."""
+    pool, table, unit = dominated_pool(fmt, d, scale, seed)
+    n, pages = 4096, 64
+    q = torch.zeros(1, hq, d)
+    q[0, :, 0] = gap + 0.11 * torch.arange(hq)
+    sm = math.log(2.0) / 6.0 / unit[0]                                # the gap in bits is q's only value
+    return (q.to(torch.bfloat16), pool, table, torch.tensor([n], dtype=torch.int32),
+            torch.arange(pages, dtype=torch.int32).expand(1, 1, pages).contiguous()), sm
+
+
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("d,hq", [(128, 1), (128, 4), (128, 8), (128, 16), (256, 4), (256, 16), (512, 2), (512, 8), (512, 16)])
+@pytest.mark.parametrize("scale", [2.0 ** -9, 2.0 ** -6, 2.0 ** -2, 256.0])
+def test_one_dominating_token(cuda, fmt, d, hq, scale):
+    """What the others add up to keeps its precision, however small they and their block scales are."""
+    fmt = FMTS[fmt]
+    for gap in (15.3, 18.4, 21.4, 25.3):
+        args, sm = dominated(fmt, d, hq, gap, scale, d + hq)
+        out, lse = S.block_decode(*[x.to(cuda) for x in args], 1, 1, fmt, sm, KS, VS)
+        check(out, lse, *args, 1, 1, fmt, sm)
+
+
+def random_case(fmt, d, hq, hk, n_q, lens, budget, seed, grow=1.0):
+    """Requests of the given lengths, FP4 block scales from 2^-9 to 448 side by side, queries `grow` times as large."""
+    g = torch.Generator().manual_seed(seed)
+    per = [(x + 63) // 64 for x in lens]
+    pool = torch.randint(0, 256, (sum(per) + 1, hk, 2, K.part_bytes(fmt, d)), generator=g, dtype=torch.uint8)
+    if fmt == K.FMT_BF16:
+        pool.view(torch.bfloat16).copy_(torch.randn(sum(per) + 1, hk, 2, K.PAGE * d, generator=g))
+    elif fmt == K.FMT_FP8:
+        pool &= 0xBF
+    else:
+        sc = pool[..., K.PAGE * d // 2:]
+        sc &= 0x0F
+        sc |= 0x28
+        pick = torch.tensor([0x01, 0x04, 0x08, 0x20, 0x38, 0x60, 0x7E], dtype=torch.uint8)
+        sc[:, :, 1] = pick[torch.randint(0, 7, sc[:, :, 1].shape, generator=g)]
+    perm = (torch.randperm(sum(per), generator=g) + 1).int()
+    table = torch.zeros(len(lens), max(per), dtype=torch.int32)
+    blocks = torch.full((len(lens), hk, budget), -1, dtype=torch.int32)
+    at = 0
+    for i, m in enumerate(per):
+        table[i, :m] = perm[at:at + m]
+        at += m
+        for h in range(hk):
+            pick = torch.randperm(m, generator=g)[:budget].int()
+            blocks[i, h, :len(pick)] = pick
+    q = (torch.randn(len(lens) * n_q, hq, d, generator=g) * 2 * grow).to(torch.bfloat16)
+    return q, pool, table, torch.tensor(lens, dtype=torch.int32), blocks
+
+
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("d", [128, 256, 512])
+@pytest.mark.parametrize("hq,hk,n_q", [(1, 1, 1), (8, 2, 1), (8, 1, 1), (8, 2, 4)])
+@pytest.mark.parametrize("grow", [1.0, 20.0])
+def test_every_scale_and_large_queries(cuda, fmt, d, hq, hk, n_q, grow):
+    fmt = FMTS[fmt]
+    args = random_case(fmt, d, hq, hk, n_q, [448, 300, 77, 1], 7, d + hq + n_q, grow)
+    out, lse = S.block_decode(*[x.to(cuda) for x in args], n_q, hk, fmt, d ** -0.5, KS, VS)
+    check(out, lse, *args, n_q, hk, fmt, d ** -0.5)
