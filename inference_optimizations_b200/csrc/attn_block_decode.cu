@@ -19,7 +19,7 @@
 // Bound by the listed pages' bytes over bf16 and E4M3 caches (16 x 16 lists of 32 pages of D = 512, bf16: 144 us, 6.7
 // TB/s; 64 x 8 lists of D = 128, E4M3: 49.5 us, 5.4 TB/s), by the conversions over FP4 caches (32 x 16 lists of 64 pages
 // of D = 512: 266 us, 4.3 TB/s), by launch and load latency for one user (8 lists of 32 pages of D = 128: 8.0 us), by the
-// path from L2 for a prefill's groups (512 x 8 lists of 32 pages, 4.3 GB, of a 35k-token request: 315 us).
+// path from L2 for a prefill's groups (512 x 8 lists of 32 pages, 4.3 GB, of a 35k-token request: 374 us).
 #include "common.cuh"
 #include "kernels.h"
 
@@ -31,14 +31,15 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 // The running maximum may lag behind the true one by kLag in the base-2 exponentials: floating point keeps its relative
-// precision, and the output is hardly ever rescaled after the first tiles.  P is rounded for the second product, to 11
-// bits (f16) or, over a bf16 cache, to 8: there the output is divided by the sum of the rounded weights (a row of ones
-// beside V), so that the rounding of a weight that dominates its row cancels; the log-sum-exp takes the sum of the
-// unrounded ones.  f16 has 2^-14 as its smallest normal number, so P carries 2^kUp there (at most 2^15 with the lag):
-// weights down to 2^-26 of the largest keep their 11 bits, smaller ones are off by at most 2^-37 of it.
+// precision, and the output is hardly ever rescaled after the first tiles.  P is rounded for the second product.  To 11
+// bits (f16) over 8-bit and 4-bit caches: f16 has 2^-14 as its smallest normal number, so P carries 2^kUp there (at most
+// 2^15 with the lag), weights down to 2^-26 of the largest keep their 11 bits, smaller ones are off by at most 2^-37 of it.
+// Over a bf16 cache both operands are bf16, whose 8 bits would be the coarsest rounding of the whole kernel: P goes in
+// as its rounding and what that left (kTerms products), 16 bits together.
 template <bool BF>
 struct Weights {
   static constexpr float kLag = BF ? 8.f : 3.f, kUp = BF ? 0.f : 12.f;
+  static constexpr int kTerms = BF ? 2 : 1;
 };
 
 template <int D_, int FMT_, int NR_>
@@ -211,8 +212,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   constexpr int NR = C::NR, ROWS = 8 * NR;
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ __align__(8) uint64_t full[kWarps][C::NS];
-  __shared__ float s_wm[kWarps][ROWS], s_wl[kWarps][ROWS], s_wn[kWarps][ROWS], s_m[ROWS], s_l[ROWS], s_n[ROWS],
-      s_qf[ROWS], s_f[8][ROWS];
+  __shared__ float s_wm[kWarps][ROWS], s_wl[kWarps][ROWS], s_m[ROWS], s_l[ROWS], s_qf[ROWS], s_f[8][ROWS];
   __shared__ int s_cnt, s_abort;
   int* s_blk = reinterpret_cast<int*>(sm + C::off_list);
   int* s_phys = s_blk + cap;
@@ -322,12 +322,6 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
     for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[t][n][k] = 0.f;
-  float accn[NR][4];                             // sum of the rounded weights, every row the same
-#pragma unroll
-  for (int n = 0; n < NR; ++n)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) accn[n][k] = 0.f;
-  constexpr uint32_t kOnes[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
   // Offsets of this lane's fragment rows: the chunk swizzle leaves NX of them (a load takes a pair of chunks), further
   // pairs lie at constant distances.
   uint32_t klane[C::NX], vlane[C::NX];
@@ -455,7 +449,6 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
         const float al = mn == -INFINITY ? 1.f : ex2((m[i] - mn) * scale[i]);
         m[i] = mn;
         l[i] *= al;
-        accn[i >> 1][i & 1] *= al;
 #pragma unroll
         for (int t = 0; t < C::MT; ++t) {
           acc[t][i >> 1][i & 1] *= al;
@@ -463,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
         }
       }
     }
-    uint32_t p[C::SUB][NR][2];
+    uint32_t p[C::SUB][NR][W::kTerms][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       const float c0 = m[2 * n] == -INFINITY ? 0.f : W::kUp - m[2 * n] * scale[2 * n];
@@ -476,7 +469,11 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
           const float p1 = ex2(fmaf(s[u][n][2 * o + 1], scale[2 * n + 1], c1));
           l[2 * n] += p0;
           l[2 * n + 1] += p1;
-          p[u][n][o] = transpose8x8(pack16<C::BF>(p0, p1));      // rows 8 n + g, tokens 2 j4, 2 j4 + 1 of the octet
+          const uint32_t w = pack16<C::BF>(p0, p1);
+          p[u][n][0][o] = transpose8x8(w);                       // rows 8 n + g, tokens 2 j4, 2 j4 + 1 of the octet
+          if constexpr (W::kTerms == 2)
+            p[u][n][W::kTerms - 1][o] = transpose8x8(
+                pack16<C::BF>(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u)));
         }
       }
     }
@@ -496,13 +493,13 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
       const uint32_t vt = vb + u * 16 * C::RB;
       if constexpr (C::BF) {
 #pragma unroll
-        for (int n = 0; n < NR; ++n) mma<true>(accn[n], kOnes, p[u][n]);
-#pragma unroll
         for (int t = 0; t < C::MT; ++t) {
           uint32_t r[4];
           ldsm4t(r, vt + vlane[t % C::NX] + t / C::NX * (C::NCH * 16));
 #pragma unroll
-          for (int n = 0; n < NR; ++n) mma<true>(acc[t][n], r, p[u][n]);
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int x = 0; x < W::kTerms; ++x) mma<true>(acc[t][n], r, p[u][n][x]);
         }
       } else if constexpr (C::FMT == kKvFp8) {
 #pragma unroll
@@ -515,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
             e4m3x4(prmt(r[e], 0u, 0x3120u), f[0], f[1]);
             e4m3x4(prmt(r[2 + e], 0u, 0x3120u), f[2], f[3]);
 #pragma unroll
-            for (int n = 0; n < NR; ++n) mma<false>(acc[2 * i + e][n], f, p[u][n]);
+            for (int n = 0; n < NR; ++n) mma<false>(acc[2 * i + e][n], f, p[u][n][0]);
           }
         }
       } else {
@@ -550,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
             for (int t = 0; t < 2; ++t) {
               const uint32_t f[4] = {v[0][2 * t], v[0][2 * t + 1], v[1][2 * t], v[1][2 * t + 1]};
 #pragma unroll
-              for (int n = 0; n < NR; ++n) mma<false>(acc[4 * i + 2 * e + t][n], f, p[u][n]);
+              for (int n = 0; n < NR; ++n) mma<false>(acc[4 * i + 2 * e + t][n], f, p[u][n][0]);
             }
           }
         }
@@ -570,7 +567,6 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
     if (g == 0) {
       s_wm[warp][r] = m[i] * scale[i] - W::kUp;
       s_wl[warp][r] = s_abort ? NAN : l[i];
-      s_wn[warp][r] = s_abort ? NAN : C::BF ? accn[i >> 1][i & 1] : l[i];
     }
     if (r < R) {
 #pragma unroll
@@ -587,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   __syncthreads();
   // ---- the CTA's partial result, in place of warp 0's
   if (tid < ROWS) {
-    float M = -INFINITY, L = 0.f, N = 0.f;
+    float M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_wm[w][tid]);
 #pragma unroll
@@ -595,11 +591,9 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
       const float f = ex2(s_wm[w][tid] - (M == -INFINITY ? 0.f : M));
       s_f[w][tid] = f;
       L += f * s_wl[w][tid];
-      N += f * s_wn[w][tid];
     }
     s_m[tid] = M;
     s_l[tid] = L;
-    s_n[tid] = N;
   }
   __syncthreads();
   for (int i = tid; i < R * (C::D / 4); i += kThreads) {
@@ -624,27 +618,24 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   // (the CTAs' statistics are fetched by as many threads, the outputs' parts all before their sum: one remote latency
   // each, not one per CTA)
   const uint32_t ao = smem_u32(sm);
-  static_assert(8 * ROWS <= kThreads && 16 * ROWS * 4 <= C::RING, "a thread per CTA and row");
+  static_assert(8 * ROWS <= kThreads && 8 * ROWS * 4 <= C::RING, "a thread per CTA and row");
   float(*s_cl)[ROWS] = reinterpret_cast<float(*)[ROWS]>(sm + C::RING);      // (the second warp's ring is free by now)
-  float(*s_cn)[ROWS] = s_cl + 8;
   if (tid < csize * ROWS) {
     const int c = tid / ROWS, r = tid % ROWS;
     s_f[c][r] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&s_m[r]), c)));
     s_cl[c][r] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&s_l[r]), c)));
-    s_cn[c][r] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&s_n[r]), c)));
   }
   __syncthreads();
   if (tid < ROWS) {
-    float M = -INFINITY, L = 0.f, N = 0.f;
+    float M = -INFINITY, L = 0.f;
     for (int c = 0; c < csize; ++c) M = fmaxf(M, s_f[c][tid]);
     const float ms = M == -INFINITY ? 0.f : M;
     for (int c = 0; c < csize; ++c) {
       const float f = ex2(s_f[c][tid] - ms);
       s_f[c][tid] = f;
       L += f * s_cl[c][tid];
-      N += f * s_cn[c][tid];
     }
-    const float inv = L == 0.f ? 0.f : (C::BF ? 1.f : a.v_scale) / N;
+    const float inv = L == 0.f ? 0.f : (C::BF ? 1.f : a.v_scale) / L;
     for (int c = 0; c < csize; ++c) s_f[c][tid] *= inv;
     if (rank == 0 && tid < R)
       a.lse[static_cast<size_t>(b * a.n_q + (r0 + tid) / G) * a.Hq + h * G + (r0 + tid) % G] =

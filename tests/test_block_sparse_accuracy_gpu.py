@@ -13,8 +13,9 @@ pytestmark = pytest.mark.gpu
 
 FMTS = {"bf16": K.FMT_BF16, "fp8": K.FMT_FP8, "nvfp4": K.FMT_NVFP4}
 KS, VS = 0.75, 1.25
-# Relative rounding of a weight for the second product: 11 bits over 8-bit and 4-bit caches, 8 bits over bf16 ones.
-UNIT = {K.FMT_BF16: 2.0 ** -8, K.FMT_FP8: 2.0 ** -11, K.FMT_NVFP4: 2.0 ** -11}
+# Relative rounding of a weight for the second product: 11 bits over 8-bit and 4-bit caches, 16 (8 and what they leave,
+# 8 more) over bf16 ones.
+UNIT = {K.FMT_BF16: 2.0 ** -16, K.FMT_FP8: 2.0 ** -11, K.FMT_NVFP4: 2.0 ** -11}
 
 
 def part_abs(pool, fmt, d):
