@@ -189,7 +189,8 @@ __device__ __forceinline__ int valid_pages(const BlockDecodeArgs& a, int unit, i
   return cnt;
 }
 
-// Power of two that brings a query row into f16's range (one warp).
+// Power of two that brings a query row's largest value into [2^14, 2^15), f16's last octave but one (one warp): values
+// down to 2^-31 of the largest keep bf16's 8 bits.
 template <int D>
 __device__ __forceinline__ float row_pow2(const __nv_bfloat16* q) {
   float amax = 0.f;
@@ -201,7 +202,7 @@ __device__ __forceinline__ float row_pow2(const __nv_bfloat16* q) {
   amax = warp_max(amax);
   int x = 0;
   if (amax > 0.f && amax < INFINITY) frexpf(amax, &x);
-  x = max(-100, min(100, x));
+  x = max(-126, x - 15);                         // (at most 128 - 15)
   return __int_as_float((x + 127) << 23);
 }
 

@@ -142,3 +142,33 @@ def test_every_scale_and_large_queries(cuda, fmt, d, hq, hk, n_q, grow):
     args = random_case(fmt, d, hq, hk, n_q, [448, 300, 77, 1], 7, d + hq + n_q, grow)
     out, lse = S.block_decode(*[x.to(cuda) for x in args], n_q, hk, fmt, d ** -0.5, KS, VS)
     check(out, lse, *args, n_q, hk, fmt, d ** -0.5)
+
+
+def lone_case(fmt, d, hq, ratio, size, seed):
+    """200 tokens whose keys have nothing in dimension 0, where every query has its largest value; the others are about
+    `ratio` of it, and the largest is `size`."""
+    g = torch.Generator().manual_seed(seed)
+    n = 200
+    k, v = torch.randn(2, n, 1, d, generator=g)
+    k[:, :, 0] = 0
+    pool = torch.zeros(5, 1, 2, K.part_bytes(fmt, d), dtype=torch.uint8)
+    table = torch.tensor([[3, 1, 4, 2]], dtype=torch.int32)
+    at = torch.arange(n)
+    K.gqa_pool_write_ref(pool, (table[0, at // 64] * 64 + at % 64).int(), k, v, fmt, KS, VS)
+    q = torch.randn(1, hq, d, generator=g) * ratio * size
+    q[:, :, 0] = size
+    sm = 2.0 / math.sqrt(d) / ratio / size
+    return (q.to(torch.bfloat16), pool, table, torch.tensor([n], dtype=torch.int32),
+            torch.arange(4, dtype=torch.int32).view(1, 1, 4)), sm
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "nvfp4"])
+@pytest.mark.parametrize("d,hq", [(128, 4), (256, 16), (512, 2), (512, 8)])
+@pytest.mark.parametrize("ratio,size", [(2.0 ** -20, 1.0), (2.0 ** -12, 2.0 ** 60), (2.0 ** -3, 2.0 ** 120)])
+def test_queries_with_one_large_value(cuda, fmt, d, hq, ratio, size):
+    """8-bit and 4-bit caches take queries through f16: the small values of a row keep their bits beside a large one, and
+    sizes up to bf16's largest stay finite."""
+    fmt = FMTS[fmt]
+    args, sm = lone_case(fmt, d, hq, ratio, size, d + hq)
+    out, lse = S.block_decode(*[x.to(cuda) for x in args], 1, 1, fmt, sm, KS, VS)
+    check(out, lse, *args, 1, 1, fmt, sm)
