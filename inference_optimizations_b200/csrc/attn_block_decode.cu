@@ -19,7 +19,7 @@
 // Bound by the listed pages' bytes over bf16 and E4M3 caches (16 x 16 lists of 32 pages of D = 512, bf16: 144 us, 6.7
 // TB/s; 64 x 8 lists of D = 128, E4M3: 49.5 us, 5.4 TB/s), by the conversions over FP4 caches (32 x 16 lists of 64 pages
 // of D = 512: 266 us, 4.3 TB/s), by launch and load latency for one user (8 lists of 32 pages of D = 128: 8.0 us), by the
-// path from L2 for a prefill's groups (512 x 8 lists of 32 pages, 4.3 GB, of a 35k-token request: 374 us).
+// path from L2 for a prefill's groups (512 x 8 lists of 32 pages, 4.3 GB, of a 35k-token request: 361 us).
 #include "common.cuh"
 #include "kernels.h"
 
@@ -35,7 +35,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // bits (f16) over 8-bit and 4-bit caches: f16 has 2^-14 as its smallest normal number, so P carries 2^kUp there (at most
 // 2^15 with the lag), weights down to 2^-26 of the largest keep their 11 bits, smaller ones are off by at most 2^-37 of it.
 // Over a bf16 cache both operands are bf16, whose 8 bits would be the coarsest rounding of the whole kernel: P goes in
-// as its rounding and what that left (kTerms products), 16 bits together.
+// as its leading 8 bits and what those left (kTerms products), 16 bits together.  Both terms of a weight that is not 0
+// are positive, so that an infinite V stays what it is.
 template <bool BF>
 struct Weights {
   static constexpr float kLag = BF ? 8.f : 3.f, kUp = BF ? 0.f : 12.f;
@@ -470,11 +471,15 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
           const float p1 = ex2(fmaf(s[u][n][2 * o + 1], scale[2 * n + 1], c1));
           l[2 * n] += p0;
           l[2 * n + 1] += p1;
-          const uint32_t w = pack16<C::BF>(p0, p1);
+          const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+          const uint32_t w = C::BF ? prmt(b0, b1, 0x7632u) : pack16<C::BF>(p0, p1);
           p[u][n][0][o] = transpose8x8(w);                       // rows 8 n + g, tokens 2 j4, 2 j4 + 1 of the octet
-          if constexpr (W::kTerms == 2)
-            p[u][n][W::kTerms - 1][o] = transpose8x8(
-                pack16<C::BF>(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u)));
+          if constexpr (W::kTerms == 2) {
+            constexpr float kLeast = 0x1p-40f;
+            p[u][n][W::kTerms - 1][o] =
+                transpose8x8(pack16<C::BF>(fmaxf(p0 - __uint_as_float(b0 & 0xffff0000u), p0 * kLeast),
+                                           fmaxf(p1 - __uint_as_float(b1 & 0xffff0000u), p1 * kLeast)));
+          }
         }
       }
     }

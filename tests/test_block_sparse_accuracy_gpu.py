@@ -172,3 +172,18 @@ def test_queries_with_one_large_value(cuda, fmt, d, hq, ratio, size):
     args, sm = lone_case(fmt, d, hq, ratio, size, d + hq)
     out, lse = S.block_decode(*[x.to(cuda) for x in args], 1, 1, fmt, sm, KS, VS)
     check(out, lse, *args, 1, 1, fmt, sm)
+
+
+@pytest.mark.parametrize("d,hq,n_q", [(128, 4, 1), (128, 4, 4), (256, 8, 1), (512, 2, 1), (512, 16, 1)])
+def test_an_infinite_value_that_every_row_sees(cuda, d, hq, n_q):
+    """Over a bf16 cache: outputs in its dimension are infinite, the others are what they are."""
+    q, pool, table, kv, blocks = random_case(K.FMT_BF16, d, hq, 1, n_q, [400, 70], 7, d + hq)
+    rb = 2 * d
+    for i, (pos, at, bits) in enumerate(((130, 5, 0x7F80), (3, d - 2, 0x7F80 - (1 << 15)))):          # inf, -inf
+        part = pool[int(table[i, pos // 64]), 0, 1].view(torch.int16)
+        part[pos % 64 * d + int(K.kv_swizzle_perm(rb)[pos % 64][2 * at]) // 2] = bits
+    out, lse = S.block_decode(*[x.to(cuda) for x in (q, pool, table, kv, blocks)], n_q, 1, K.FMT_BF16, 0.3, KS, VS)
+    want, wlse = S.block_decode_ref(q, pool, table, kv, blocks, n_q, 1, K.FMT_BF16, 0.3, KS, VS, None, torch.float64)
+    odd = ~torch.isfinite(want)
+    assert odd.sum() == 2 * n_q * hq and torch.equal(out.cpu().double()[odd], want[odd])
+    assert torch.equal(torch.isfinite(out.cpu()), ~odd)
