@@ -43,9 +43,12 @@ struct Weights {
   static constexpr int kTerms = BF ? 2 : 1;
 };
 
-template <int D_, int FMT_, int NR_>
+template <int D_, int FMT_, int NR_, bool GROUP_>
 struct Cfg {
   static constexpr int D = D_, FMT = FMT_, NR = NR_;       // NR: groups of 8 query rows
+  // Several tokens of a request in one list: a row of V may be seen by some of the query rows only.  A form of its own,
+  // because the little that it adds costs the other one its schedule (D = 512, FP4, 32 x 16 x 64 pages: 264 / 275 us).
+  static constexpr bool GROUP = GROUP_;
   static constexpr bool BF = FMT == kKvBf16;
   static constexpr int RB = BF ? 2 * D : FMT == kKvFp8 ? D : D / 2;       // bytes of a row
   static constexpr int SC = FMT == kKvNvfp4 ? D / 16 : 0;                 // block scale bytes of a row
@@ -165,6 +168,45 @@ __device__ __forceinline__ uint32_t q_pair(const __nv_bfloat16* q, float f) {
   return pack16<false>(__uint_as_float(raw << 16) * f, __uint_as_float(raw & 0xffff0000u) * f);
 }
 
+// Words of stored V rows (block scales for an FP4 cache): the value with everything that is not finite cleared.
+template <int FMT>
+__device__ __forceinline__ uint32_t finite_word(uint32_t w) {
+  if constexpr (FMT == kKvBf16) {
+    if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+    if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
+  } else {                                       // E4M3: NaN only
+    w &= ~(__vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu));
+  }
+  return w;
+}
+// Clears what is not finite in the V rows [lo, hi) of a tile (one warp; a call, so that the main loop's registers and
+// schedule do not depend on it).
+template <class C>
+__device__ __noinline__ void clear_odd(uint8_t* tile, int lo, int hi, int* found) {
+  constexpr int ZB = C::FMT == kKvNvfp4 ? C::SC : C::RB;
+  uint8_t* z = tile + (C::FMT == kKvNvfp4 ? C::ST * C::RB : 0);
+  for (int i = max(0, lo) * ZB + 4 * lane_id(); i < min(C::ST, hi) * ZB; i += 128) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(z + i), f = finite_word<C::FMT>(w);
+    if (w != f) {
+      *reinterpret_cast<uint32_t*>(z + i) = f;
+      *found = 1;
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+// Value d of V row `row` of a page if it is not finite, else 0.
+template <class C>
+__device__ __forceinline__ float not_finite(const uint8_t* part, int row, int d) {
+  if constexpr (C::BF) {
+    const uint32_t v = *reinterpret_cast<const uint16_t*>(part + swz<C>(row, d / 8) + 2 * (d % 8));
+    return (v & 0x7f80u) == 0x7f80u ? __uint_as_float(v << 16) : 0.f;
+  } else {
+    const uint8_t v = C::FMT == kKvFp8 ? part[swz<C>(row, d / 16) + d % 16] : part[kPage * C::RB + row * C::SC + d / 16];
+    return (v & 0x7fu) == 0x7fu ? NAN : 0.f;
+  }
+}
+
 // The list entries of one unit that name a page of the request and the pool, by one warp: logical pages in s_blk,
 // physical pages in s_phys; returns their number.
 __device__ __forceinline__ int valid_pages(const BlockDecodeArgs& a, int unit, int prow, int len, int* s_blk,
@@ -215,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ __align__(8) uint64_t full[kWarps][C::NS];
   __shared__ float s_wm[kWarps][ROWS], s_wl[kWarps][ROWS], s_m[ROWS], s_l[ROWS], s_qf[ROWS], s_f[8][ROWS];
-  __shared__ int s_cnt, s_abort;
+  __shared__ int s_cnt, s_abort, s_odd, s_odd_any;
   int* s_blk = reinterpret_cast<int*>(sm + C::off_list);
   int* s_phys = s_blk + cap;
   const int tid = threadIdx.x, warp = warp_id(), lane = lane_id();
@@ -232,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
            static_cast<size_t>(h * G + (r0 + r) % G) * C::D;
   };
   if (tid == 0) {
-    s_abort = 0;
+    s_abort = s_odd = s_odd_any = 0;
     for (int i = 0; i < kWarps * C::NS; ++i) mbar_init(&full[0][0] + i, 1);
     fence_mbar_init();
   }
@@ -493,6 +535,10 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
       fence_proxy_async_smem();
       __syncwarp();
     }
+    // A row of V that later tokens of the group see and earlier ones do not meets weights of 0 in this product, and 0 x inf
+    // is NaN: values that are not finite are taken out here and added at the end, to the rows that see them.
+    if constexpr (C::GROUP)
+      if (base + C::ST - 1 > q0) clear_odd<C>(vp, q0 + 1 - base, len - base, &s_odd);
     const uint32_t vb = smem_u32(vp);
 #pragma unroll
     for (int u = 0; u < C::SUB; ++u) {
@@ -628,8 +674,12 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   float(*s_cl)[ROWS] = reinterpret_cast<float(*)[ROWS]>(sm + C::RING);      // (the second warp's ring is free by now)
   if (tid < csize * ROWS) {
     const int c = tid / ROWS, r = tid % ROWS;
-    s_f[c][r] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&s_m[r]), c)));
-    s_cl[c][r] = __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&s_l[r]), c)));
+    const uint32_t vm = ld_cluster_u32(mapa_shared(smem_u32(&s_m[r]), c));
+    const uint32_t vl = ld_cluster_u32(mapa_shared(smem_u32(&s_l[r]), c));
+    const uint32_t odd = C::GROUP ? ld_cluster_u32(mapa_shared(smem_u32(&s_odd), c)) : 0u;
+    s_f[c][r] = __uint_as_float(vm);
+    s_cl[c][r] = __uint_as_float(vl);
+    if (odd != 0u) s_odd_any = 1;
   }
   __syncthreads();
   if (tid < ROWS) {
@@ -666,6 +716,18 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
         o.w += f * v[c].w;
       }
     }
+    if (C::GROUP && s_odd_any) {                           // V that is not finite, of the group's own tokens up to this row's
+      const int last = min(len - 1, q0 + (r0 + row) / G);
+      for (int pos = max(0, q0 + 1); pos <= last; ++pos)
+        for (int j = 0; j < s_cnt; ++j)
+          if (s_blk[j] == pos / kPage) {
+            const uint8_t* part = a.pool + (static_cast<size_t>(s_phys[j]) * a.Hk + h) * (2 * C::PART) + C::PART;
+            o.x += not_finite<C>(part, pos % kPage, d);
+            o.y += not_finite<C>(part, pos % kPage, d + 1);
+            o.z += not_finite<C>(part, pos % kPage, d + 2);
+            o.w += not_finite<C>(part, pos % kPage, d + 3);
+          }
+    }
     uint2 raw;
     raw.x = pack16<true>(o.x, o.y);
     raw.y = pack16<true>(o.z, o.w);
@@ -675,9 +737,8 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   if (csize > 1) cluster_sync_all();             // a CTA's partial results are read until here
 }
 
-template <int D, int FMT, int NR>
-cudaError_t launch_r(const BlockDecodeArgs& a, int rgroups, cudaStream_t s) {
-  using C = Cfg<D, FMT, NR>;
+template <class C>
+cudaError_t launch_c(const BlockDecodeArgs& a, int rgroups, cudaStream_t s) {
   // Few lists: each is split over a cluster, as far as the SMs have room for all its CTAs at once and a CTA keeps two
   // pages.
   const int units = a.B * a.Hk * rgroups;
@@ -699,6 +760,11 @@ cudaError_t launch_r(const BlockDecodeArgs& a, int rgroups, cudaStream_t s) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, k, a, cs, a.budget, rgroups);
+}
+
+template <int D, int FMT, int NR>
+cudaError_t launch_r(const BlockDecodeArgs& a, int rgroups, cudaStream_t s) {
+  return a.n_q > 1 ? launch_c<Cfg<D, FMT, NR, true>>(a, rgroups, s) : launch_c<Cfg<D, FMT, NR, false>>(a, rgroups, s);
 }
 
 template <int D, int FMT>

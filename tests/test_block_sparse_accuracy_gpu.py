@@ -55,7 +55,8 @@ def check(out, lse, q, pool, table, kv, blocks, n_q, hk, fmt, sm):
     tol = want.abs() * 2.0 ** -8 + mag * (UNIT[fmt] + 2 * ds) + total * tiny + 1e-30
     got = out.cpu().double()
     off = (got - want).abs()
-    assert ((off <= tol) | (want.isnan() & got.isnan())).all(), f"{(off / tol).max()} of the bound"
+    same = (got == want) | (want.isnan() & got.isnan())               # (infinities and NaN)
+    assert ((off <= tol) | same).all(), f"{(off / tol).max()} of the bound"
     near = (lse.cpu().double() - wlse).abs() <= ds[..., 0] + 2.0 ** -20 * (1 + wlse.abs())
     assert (near | (lse.cpu() == wlse)).all()                         # (a row that sees nothing: -inf)
 
@@ -187,3 +188,32 @@ def test_an_infinite_value_that_every_row_sees(cuda, d, hq, n_q):
     odd = ~torch.isfinite(want)
     assert odd.sum() == 2 * n_q * hq and torch.equal(out.cpu().double()[odd], want[odd])
     assert torch.equal(torch.isfinite(out.cpu()), ~odd)
+
+
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("d,hq,hk,n_q", [(128, 8, 2, 4), (128, 2, 2, 16), (256, 8, 2, 4), (256, 3, 3, 5), (512, 4, 2, 4),
+                                         (512, 16, 4, 4)])
+def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(cuda, fmt, d, hq, hk, n_q):
+    """A verify group's own tokens, on one page and on two, with infinite or NaN V (over 8-bit and 4-bit caches NaN)."""
+    fmt = FMTS[fmt]
+    lens = [n_q, 64 + 2, 200, 64 * 5, 64 * 4 + n_q - 1, 64 * 7 + 2]
+    q, pool, table, kv, blocks = random_case(fmt, d, hq, hk, n_q, lens, 8, d + n_q)
+    for i, n in enumerate(lens):
+        for pos, at, kind in ((n - 1, 3, 0x7F80), (n - 2, 3, 0xFF80), (n - 2, d - 1, 0x7FC0), (n - n_q // 2, 40, 0xFF80)):
+            page, off = int(table[i, pos // 64]), pos % 64
+            part = pool[page, hk - 1, 1]
+            rb = K.row_bytes(fmt, d)
+            per = 8 if fmt == K.FMT_BF16 else 16
+            chunk = int(K.kv_swizzle_perm(rb)[off][at // per * 16]) if fmt != K.FMT_NVFP4 else 0
+            if fmt == K.FMT_BF16:
+                part[off * rb:(off + 1) * rb].view(torch.int16)[chunk // 2 + at % per] = kind - (1 << 16 if kind >= 1 << 15 else 0)
+            elif fmt == K.FMT_FP8:
+                part[off * rb + chunk + at % per] = 0x7F if kind != 0xFF80 else 0xFF
+            else:
+                part[64 * rb + off * (d // 16) + at // 16] = 0x7F
+    blocks[5, :, :] = -1
+    blocks[5, :, 0] = 6                                               # a list without the group's second page
+    out, lse = S.block_decode(*[x.to(cuda) for x in (q, pool, table, kv, blocks)], n_q, hk, fmt, d ** -0.5, KS, VS)
+    want, _ = S.block_decode_ref(q, pool, table, kv, blocks, n_q, hk, fmt, d ** -0.5, KS, VS, None, torch.float64)
+    assert torch.equal(out.isfinite().cpu(), want.isfinite()) and not want.isfinite().all()
+    check(out, lse, q, pool, table, kv, blocks, n_q, hk, fmt, d ** -0.5)
