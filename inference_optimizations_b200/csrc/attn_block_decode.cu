@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
   bool ival = false;
   auto issue = [&](int slot) {
     uint8_t* dst = ring + slot * C::SLOT;
-    mbar_expect_tx(&full[warp][slot], C::SLOT);
+    mbar_expect_tx(&full[warp][slot], C::SLOT + a.never_bytes);
     const int in = itile % C::TPP;
     if (!ival) {
       isrc = a.pool + (static_cast<size_t>(s_phys[itile / C::TPP]) * a.Hk + h) * (2 * C::PART) + in * (C::ST * C::RB);
@@ -609,7 +609,16 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
     if (lane == 0 && 2 * k + 1 + C::NS < 2 * nk && !s_abort) issue(slot);
     if (++slot == C::NS) { slot = 0; phase ^= 1; }
   }
-  // ---- partial result of the warp in place of its ring (idle: every issued copy was waited for)
+  // A wait that ran out in some warp: this one may have copies under way that it did not wait for.  It waits for the last
+  // of each slot, with the same limit, before anything takes their place or the CTA ends; the group's result is NaN.
+  const bool lost = __any_sync(0xffffffffu, *const_cast<volatile int*>(&s_abort));
+  bool idle = true;
+  if (lost) {
+    const int issued = __shfl_sync(0xffffffffu, 2 * ((itile - t0) / step) + (ival ? 1 : 0), 0);
+    for (int q = max(0, issued - C::NS); idle && q < issued; ++q)
+      idle = __all_sync(0xffffffffu, mbar_wait(&full[warp][q % C::NS], (q / C::NS) & 1, nullptr, a.status, kTimeoutProducer));
+  }
+  // ---- partial result of the warp in place of its ring, which is idle
   float* wO = reinterpret_cast<float*>(ring);                     // [ROWS][DP]
 #pragma unroll
   for (int i = 0; i < 2 * NR; ++i) {
@@ -618,9 +627,9 @@ __global__ void __launch_bounds__(kThreads, C::RES) block_decode_kernel(const Bl
     const int r = 8 * (i >> 1) + 2 * j4 + (i & 1);
     if (g == 0) {
       s_wm[warp][r] = m[i] * scale[i] - W::kUp;
-      s_wl[warp][r] = s_abort ? NAN : l[i];
+      s_wl[warp][r] = lost ? NAN : l[i];
     }
-    if (r < R) {
+    if (r < R && idle) {
 #pragma unroll
       for (int t = 0; t < C::MT; ++t) {
         int d, dn;                               // values of rows g, g + 8 of the tile

@@ -415,9 +415,10 @@ std::tuple<at::Tensor, at::Tensor> block_decode(const at::Tensor& q, const at::T
                   const at::Tensor& page_table, c10::optional<at::Tensor> req_idx, const at::Tensor& kv_len,
                   const at::Tensor& blocks, c10::optional<at::Tensor> out_given, c10::optional<at::Tensor> lse_given,
                   c10::optional<at::Tensor> status, int64_t n_q, int64_t Hk, int64_t fmt, double sm_scale,
-                  double k_scale, double v_scale) {
+                  double k_scale, double v_scale, int64_t never_bytes) {
   block_groups(q, page_table, req_idx, kv_len, n_q, Hk);
   const int64_t D = q.size(2), B = kv_len.size(0);
+  TORCH_CHECK(never_bytes >= 0 && never_bytes <= 1024, "never_bytes");
   block_pool(pool, fmt, Hk, D);
   req(blocks, at::kInt, "blocks");
   const at::cuda::CUDAGuard g(q.device());
@@ -460,6 +461,7 @@ std::tuple<at::Tensor, at::Tensor> block_decode(const at::Tensor& q, const at::T
   a.pages = static_cast<int>(pool.size(0));
   a.budget = static_cast<int>(blocks.size(2));
   a.fmt = static_cast<int>(fmt);
+  a.never_bytes = static_cast<int>(never_bytes);
   a.sm_scale = static_cast<float>(sm_scale);
   a.k_scale = static_cast<float>(k_scale);
   a.v_scale = static_cast<float>(v_scale);
@@ -1185,7 +1187,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("block_append", &block_append);
   m.def("block_summarize", &block_summarize);
   m.def("block_select", &block_select);
-  m.def("block_decode", &block_decode);
+  m.def("block_decode", &block_decode, py::arg("q"), py::arg("pool"), py::arg("page_table"), py::arg("req_idx"),
+        py::arg("kv_len"), py::arg("blocks"), py::arg("out"), py::arg("lse"), py::arg("status"), py::arg("n_q"),
+        py::arg("hk"), py::arg("fmt"), py::arg("sm_scale"), py::arg("k_scale"), py::arg("v_scale"),
+        py::arg("never_bytes") = 0);
   m.def("act_quant", &act_quant);
   m.def("splitk_reduce", &splitk_reduce);
   m.def("ep_dispatch", &ep_dispatch);

@@ -399,6 +399,7 @@ struct BlockDecodeArgs {
   float* lse;              // fp32 [B * n_q, Hq], natural log of the softmax's sum; -inf where nothing is visible
   int* status;             // or null
   int B, n_q, Hq, Hk, D, rows, pt_stride, pages, budget, fmt;
+  int never_bytes;         // 0; bytes that every copy is awaited for and does not bring: the wait limit runs out (tests)
   float sm_scale, k_scale, v_scale;
 };
 cudaError_t block_decode(const BlockDecodeArgs& a, cudaStream_t s);

@@ -1,0 +1,38 @@
+"""A copy that does not arrive: `block_decode` gives up after its wait limit (~2 s), waits for its other copies with the
+same limit, marks the group's output NaN, records a status and leaves the context usable.  No copy is really lost: every
+barrier awaits a few bytes more than its copy brings."""
+import time
+
+import pytest
+import torch
+
+from inference_optimizations_b200.ops import block_sparse as S
+from inference_optimizations_b200.ops import kvcache as K
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("fmt,d,hq,n_q,pages", [(K.FMT_BF16, 128, 4, 1, 40), (K.FMT_FP8, 256, 4, 4, 3),
+                                                (K.FMT_NVFP4, 512, 2, 1, 1), (K.FMT_BF16, 512, 2, 8, 24)])
+def test_decode_gives_up_on_a_copy_that_does_not_arrive(cuda, fmt, d, hq, n_q, pages):
+    from inference_optimizations_b200._ext import ext
+    from inference_optimizations_b200.parallel import health as HL
+    pool = torch.zeros(pages + 1, 1, 2, K.part_bytes(fmt, d), dtype=torch.uint8, device=cuda)
+    table = torch.arange(1, pages + 1, dtype=torch.int32, device=cuda)[None].repeat(2, 1)
+    kv = torch.tensor([pages * 64, 0], dtype=torch.int32, device=cuda)           # the second group has nothing to wait for
+    blocks = torch.arange(pages, dtype=torch.int32, device=cuda).repeat(2, 1, 1)
+    q = torch.randn(2 * n_q, hq, d, device=cuda).to(torch.bfloat16)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    args = (q, pool, table, None, kv, blocks, None, None, status, n_q, 1, fmt, 0.1, 1.0, 1.0)
+    t0 = time.time()
+    out, lse = ext().block_decode(*args, never_bytes=16)
+    torch.cuda.synchronize()
+    assert time.time() - t0 < 15
+    assert status.item() == 1 and out[:n_q].isnan().all() and lse[:n_q].isnan().all()
+    assert not out[n_q:].any() and (lse[n_q:] == -float("inf")).all()
+    with pytest.raises(HL.DeviceWaitTimeout):
+        HL.check_status([status])
+    status.zero_()
+    out, lse = ext().block_decode(*args)
+    assert status.item() == 0 and not out.any() and lse[:n_q].isfinite().all()
+    assert torch.equal(S.block_decode(q, pool, table, kv, blocks, n_q, 1, fmt, 0.1)[1], lse)
