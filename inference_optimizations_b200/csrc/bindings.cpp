@@ -374,6 +374,7 @@ std::tuple<at::Tensor, at::Tensor> block_select(const at::Tensor& q, const at::T
   const int64_t D = q.size(2), B = kv_len.size(0);
   TORCH_CHECK(D == 128 || D == 256 || D == 512, "head_dim 128, 256 or 512, got ", num(D));
   block_bounds(codes, scale, codes.dim() > 0 ? codes.size(0) : 0, Hk, D);
+  TORCH_CHECK(codes.size(0) >= 1, "codes of at least one page");      // (a page outside the pool is scored as page 0)
   TORCH_CHECK(sink >= 0 && local >= 1 && budget >= sink + local + 1 && budget <= iob::kBlockMaxList,
               "budget must hold sink + local + 1 pages and at most ", num(iob::kBlockMaxList));
   const at::cuda::CUDAGuard g(q.device());

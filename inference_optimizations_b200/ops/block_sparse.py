@@ -150,6 +150,8 @@ def block_select(q: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, page
     _check_groups(q, page_table, kv_len, n_q, hk)
     if sink < 0 or local < 1 or not sink + local + 1 <= budget <= MAX_LIST:
         raise RuntimeError(f"budget must hold sink + local + 1 pages and at most {MAX_LIST}")
+    if codes.shape[0] < 1:
+        raise RuntimeError("codes of at least one page")
     if page_table.shape[1] > MAX_PAGES:
         raise RuntimeError(f"page_table wider than {MAX_PAGES}")
     blocks.fill_(-1)

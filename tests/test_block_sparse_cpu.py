@@ -150,6 +150,14 @@ def test_refusals():
                        128, 1e-6, True, 1.0, 0.0)
 
 
+
+def test_selection_over_bounds_of_no_page_is_refused():
+    q, pool, table, codes, sc, *_ = session(K.FMT_BF16, 64 * 9)
+    for n in (64 * 9, 64):                                  # with candidates to score and without
+        with pytest.raises(RuntimeError, match="at least one page"):
+            S.block_select(q[-1:], codes[:0], sc[:0], table, torch.tensor([n], dtype=torch.int32), 1, 2, 3)
+
+
 # ------------------------------------------------------------------------------------------------ engine
 def _engine(**kw):
     from inference_optimizations_b200.config import EngineConfig

@@ -1,4 +1,6 @@
-"""A copy that does not arrive: `block_decode` gives up after its wait limit (~2 s), waits for its other copies with the
+"""What `block_decode` and `block_select` do at their limits.
+
+A copy that does not arrive: `block_decode` gives up after its wait limit (~2 s), waits for its other copies with the
 same limit, marks the group's output NaN, records a status and leaves the context usable.  No copy is really lost: every
 barrier awaits a few bytes more than its copy brings."""
 import time
@@ -36,3 +38,12 @@ def test_decode_gives_up_on_a_copy_that_does_not_arrive(cuda, fmt, d, hq, n_q, p
     out, lse = ext().block_decode(*args)
     assert status.item() == 0 and not out.any() and lse[:n_q].isfinite().all()
     assert torch.equal(S.block_decode(q, pool, table, kv, blocks, n_q, 1, fmt, 0.1)[1], lse)
+
+
+def test_selection_over_bounds_of_no_page_is_refused(cuda):
+    codes, sc = S.alloc_bounds(0, 2, 128, cuda)
+    q = torch.zeros(1, 4, 128, dtype=torch.bfloat16, device=cuda)
+    table = torch.zeros(1, 9, dtype=torch.int32, device=cuda)
+    for n in (64 * 9, 64):
+        with pytest.raises(RuntimeError, match="at least one page"):
+            S.block_select(q, codes, sc, table, torch.tensor([n], dtype=torch.int32, device=cuda), 1, 2, 3)
