@@ -24,6 +24,7 @@ from ..models.gqa import GQAKVCache, GQAModel, StepTensors
 from ..ops import attention as A
 from ..ops import basic as B
 from ..ops import kvcache as K
+from ..parallel.health import check_status
 from .scheduler import SamplingParams, Batch, Request, Segment
 
 KINDS = ("global", "swa", "draft")
@@ -163,6 +164,7 @@ class GQARunner:
         self.out_ids = torch.zeros(max_tok, dtype=torch.int32, device=device)
         pin = self.device.type == "cuda"
         self.out_host = torch.zeros(max_tok, dtype=torch.int32, pin_memory=pin)
+        self.status_host = torch.zeros(1, dtype=torch.int32, pin_memory=pin)
         if self.spec:
             self._init_spec()
 
@@ -415,13 +417,23 @@ class GQARunner:
         self._timed(fn)
         n = len(segs)
         self.out_host[:n].copy_(self.out_ids[:n], non_blocking=True)
-        if self.device.type == "cuda":
-            torch.cuda.current_stream().synchronize()
+        self._finish_step()
         res = {r.rid: [int(self.out_host[i])] for i, r in enumerate(reqs)}
         if self.spec:
             self._keep_draft_inputs(reqs)
         self._trim([Segment(r, r.kv_len, [0], False) for r in reqs])
         return res
+
+    def _finish_step(self) -> None:
+        """Wait for a decode / verify step's tokens.  Raises `DeviceWaitTimeout` if a wait of block-sparse attention ran
+        out (the step's tokens are then worthless); the word is cleared, no request has moved, the step may be repeated."""
+        if self.kv.sparse:
+            self.status_host.copy_(self.kv.sparse_status, non_blocking=True)
+        if self.device.type == "cuda":
+            torch.cuda.current_stream().synchronize()
+        if self.kv.sparse and int(self.status_host[0]):
+            self.kv.sparse_status.zero_()
+            check_status([self.status_host])
 
     def draft_row(self, r) -> int:
         """Row of the stored target hiddens that a plain decode step of `r` fills: the next draft extend covers
@@ -667,8 +679,7 @@ class GQARunner:
         self._timed(self._spec_fn(bucket))
         n = len(reqs)
         self.spec_out_host[:n].copy_(self.spec_out[:n], non_blocking=True)
-        if self.device.type == "cuda":
-            torch.cuda.current_stream().synchronize()
+        self._finish_step()
         res = {}
         for i, r in enumerate(reqs):
             o = self.spec_out_host[i].tolist()

@@ -225,3 +225,27 @@ def test_engine_refuses_what_it_cannot_serve():
                dict(sparse_pages=4, model="tiny_mla", kv_dtype="nvfp4")):
         with pytest.raises(ValueError):
             _engine(**kw)
+
+
+@pytest.mark.parametrize("spec", [False, True])
+def test_engine_reports_a_wait_that_ran_out(spec):
+    """A status word of the attention ends the step with an error; the step can be repeated."""
+    from inference_optimizations_b200.engine.scheduler import SamplingParams
+    from inference_optimizations_b200.parallel.health import DeviceWaitTimeout
+    torch.manual_seed(3)
+    prompts = [torch.randint(1, 500, (n,)).tolist() for n in (260, 70)]
+    want = _engine(sparse_pages=4, spec=spec).generate(prompts, SamplingParams(max_new_tokens=8))
+    eng = _engine(sparse_pages=4, spec=spec)
+    reqs = [eng.add_request(p, SamplingParams(max_new_tokens=8)) for p in prompts]
+    while len(eng.sched.running) < 2 or any(len(r.output) < 2 for r in reqs):
+        eng.step()
+    for _ in range(2):
+        eng.runner.kv.sparse_status.fill_(1)
+        before = [list(r.output) for r in reqs]
+        with pytest.raises(DeviceWaitTimeout):
+            eng.step()
+        assert [r.output for r in reqs] == before
+        eng.step()
+    while eng.has_work():
+        eng.step()
+    assert [r.output for r in reqs] == want
