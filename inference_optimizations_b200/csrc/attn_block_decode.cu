@@ -768,6 +768,10 @@ cudaError_t launch_c(const BlockDecodeArgs& a, int rgroups, cudaStream_t s) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  while (cs > 1 && !cluster_fits(k, cfg)) {
+    attr[0].val.clusterDim.x = --cs;
+    cfg.gridDim.x = static_cast<unsigned>(units) * cs;
+  }
   return cudaLaunchKernelEx(&cfg, k, a, cs, a.budget, rgroups);
 }
 

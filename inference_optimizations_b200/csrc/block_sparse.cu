@@ -814,6 +814,10 @@ cudaError_t select_launch_v(const BlockSelectArgs& a, int cs, cudaStream_t s) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  while (cs > 1 && !cluster_fits(k, cfg)) {
+    attr[0].val.clusterDim.x = --cs;
+    cfg.gridDim.x = static_cast<unsigned>(a.B) * cs;
+  }
   return cudaLaunchKernelEx(&cfg, k, a, cs);
 }
 template <int D, bool R8>

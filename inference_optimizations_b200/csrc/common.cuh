@@ -190,6 +190,15 @@ __device__ __forceinline__ void fence_proxy_async_cluster() {
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Whether a cluster of the launch's size fits at all (host): its CTAs need SMs of one GPC, of which an SM partition of
+// the device may hold few.
+template <typename K>
+inline bool cluster_fits(K kernel, const cudaLaunchConfig_t& cfg) {
+  int n = 0;
+  const bool ok = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0;
+  if (!ok) (void)cudaGetLastError();
+  return ok;
+}
 // Wait on a local mbarrier whose arrivals may come from peer CTAs (acquire at cluster scope); bounded like mbar_wait.
 __device__ __forceinline__ bool mbar_try_wait_cl(uint64_t* bar, uint32_t parity, uint32_t hint_ns = 20000) {
   uint32_t ok;
