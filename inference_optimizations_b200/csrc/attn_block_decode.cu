@@ -753,13 +753,14 @@ cudaError_t launch_c(const BlockDecodeArgs& a, int rgroups, cudaStream_t s) {
   const int units = a.B * a.Hk * rgroups;
   int cs = 1;
   while (cs < 8 && units * (cs + 1) <= 148 * C::RES && a.budget >= 2 * (cs + 1)) ++cs;
-  const int smem = C::smem(a.budget);
+  // (the limit is the longest list's, the same in every call: calls of several host threads do not lower it)
+  static_assert(C::smem(kBlockMaxList) + 4096 <= 227 * 1024, "the longest list fits beside the rings");
   auto k = block_decode_kernel<C>;
-  IOB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  IOB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(kBlockMaxList)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(units) * cs);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = C::smem(a.budget);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

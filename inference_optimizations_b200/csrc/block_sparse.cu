@@ -798,14 +798,15 @@ cudaError_t summarize_launch(const BlockAppendArgs& a, const int* pages, int n, 
 }
 template <int D, bool R8, int NT, int PP, int RES>
 cudaError_t select_launch_v(const BlockSelectArgs& a, int cs, cudaStream_t s) {
-  const int smem = 16 * (2 * D + 64) + 4 * a.pt_stride;
+  // (the limit is the widest table's, the same in every call: calls of several host threads do not lower it)
+  constexpr int kRows = 16 * (2 * D + 64), kMost = kRows + 4 * kBlockSelectMaxPages;
+  static_assert(kMost + 4096 <= 227 * 1024, "the widest table's keys fit");
   auto k = block_select_kernel<D, R8, NT, PP, RES>;
-  if (smem > 48 * 1024)
-    IOB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  IOB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.B) * cs, a.Hk);
   cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = kRows + 4 * a.pt_stride;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

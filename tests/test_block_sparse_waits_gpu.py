@@ -47,3 +47,34 @@ def test_selection_over_bounds_of_no_page_is_refused(cuda):
     for n in (64 * 9, 64):
         with pytest.raises(RuntimeError, match="at least one page"):
             S.block_select(q, codes, sc, table, torch.tensor([n], dtype=torch.int32, device=cuda), 1, 2, 3)
+
+
+@pytest.mark.parametrize("fmt,d,hq,n_q", [(K.FMT_BF16, 512, 2, 1), (K.FMT_FP8, 128, 8, 2), (K.FMT_NVFP4, 512, 2, 8),
+                                          (K.FMT_BF16, 256, 8, 2)])
+def test_long_and_short_lists_from_two_threads(cuda, fmt, d, hq, n_q):
+    """The longest list (every form's largest shared memory) and the shortest one, called in turn by two host threads."""
+    import threading
+    pool = torch.zeros(9, 1, 2, K.part_bytes(fmt, d), dtype=torch.uint8, device=cuda)
+    codes, sc = S.alloc_bounds(9, 1, d, cuda)
+    q = torch.randn(n_q, hq, d, device=cuda).to(torch.bfloat16)
+    torch.cuda.synchronize()
+    failed = []
+
+    def calls(width, budget):
+        try:
+            table = torch.ones(1, width, dtype=torch.int32, device=cuda)
+            kv = torch.tensor([8 * 64], dtype=torch.int32, device=cuda)
+            for _ in range(50):
+                blocks, count = S.block_select(q, codes, sc, table, kv, n_q, 1, budget)
+                out, lse = S.block_decode(q, pool, table, kv, blocks, n_q, 1, fmt, 0.1)
+            torch.cuda.synchronize()
+            if count.item() != min(8, budget) or out.any() or not lse.isfinite().all():
+                failed.append((width, budget))
+        except RuntimeError as e:
+            failed.append(e)
+    threads = [threading.Thread(target=calls, args=a) for a in ((S.MAX_PAGES, S.MAX_LIST), (9, 3))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
