@@ -521,9 +521,9 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// fp32 -> unsigned key of the same order (the scores are never NaN).
+// fp32 -> unsigned key of the same order (the scores are never NaN; -0, which a product that underflows can be, is 0).
 __device__ __forceinline__ uint32_t order_key(float f) {
-  const uint32_t b = __float_as_uint(f);
+  const uint32_t b = __float_as_uint(__fadd_rn(f, 0.f));      // (an addition that is not fused with the product)
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
