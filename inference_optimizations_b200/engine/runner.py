@@ -89,7 +89,7 @@ class GQARunner:
             raise ValueError("kv_dtype 'kvmix' (FP8 + NVFP4 latent rows in one page space) is an MLA-family pool")
         sparse = None
         if ecfg.sparse_pages:
-            from ..ops.block_sparse import HEAD_DIMS, MAX_LIST
+            from ..ops.block_sparse import HEAD_DIMS, MAX_LIST, MAX_PAGES
             sparse = (ecfg.sparse_pages, ecfg.sparse_sink, ecfg.sparse_local)
             rows = (4 if ecfg.spec else 1) * (cfg.num_q_heads // cfg.num_kv_heads_global)
             if not (sparse[1] >= 0 and sparse[2] >= 1 and sparse[1] + sparse[2] + 1 <= sparse[0] <= MAX_LIST):
@@ -97,6 +97,8 @@ class GQARunner:
             if cfg.head_dim_global not in HEAD_DIMS or rows > 16:
                 raise ValueError(f"block-sparse decode needs global head_dim in {HEAD_DIMS} and at most 16 query rows "
                                  f"per kv head (verify tokens x group), got {cfg.head_dim_global}, {rows}")
+            if GQAKVCache.table_pages(max_seq + 64) > MAX_PAGES:
+                raise ValueError(f"block-sparse decode ranks up to {MAX_PAGES} pages of a request, max_seq is {max_seq}")
         self.cfg, self.ecfg, self.device = cfg, ecfg, torch.device(device)
         self.tp, self.tp_rank = tp, tp_rank
         self.max_seq = max_seq

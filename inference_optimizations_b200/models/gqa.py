@@ -370,7 +370,7 @@ class GQAKVCache:
         self.device = torch.device(device)
         self.max_pos = max_seq + 64
         self.k_scale, self.v_scale = k_scale, v_scale
-        max_pages = (max_seq + 63) // 64 + 1
+        max_pages = self.table_pages(max_seq)
         self.pools = []
         self.kinds = []
         self.sparse = sparse
@@ -399,6 +399,11 @@ class GQAKVCache:
         self._ws = {}
         self.ext_status = torch.zeros(1, dtype=torch.int32, device=device)
         self.sparse_status = torch.zeros(1, dtype=torch.int32, device=device)
+
+    @staticmethod
+    def table_pages(max_seq: int) -> int:
+        """Width of the page tables."""
+        return (max_seq + 63) // 64 + 1
 
     def workspace(self, d: int, hk: int, lane: int = 0) -> Optional[A.DecodeWorkspace]:
         """The decode lane's reserved split workspace; the prefill lane (lane 1) gets None, so each call allocates

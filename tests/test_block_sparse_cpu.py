@@ -249,3 +249,14 @@ def test_engine_reports_a_wait_that_ran_out(spec):
     while eng.has_work():
         eng.step()
     assert [r.output for r in reqs] == want
+
+
+def test_engine_refuses_tables_wider_than_the_selection():
+    from inference_optimizations_b200.config import EngineConfig
+    from inference_optimizations_b200.engine.engine import Engine
+    ecfg = EngineConfig(model="tiny_gqa", device="cpu", kv_dtype="bf16", max_running=1, chunked_prefill=64,
+                        cuda_graphs=False, sparse_pages=8)
+    widest = 64 * (S.MAX_PAGES - 2)                          # one page of growth, one spare entry
+    assert Engine(ecfg, max_seq=widest, global_pages=8).runner.kv.tables["global"].dev.shape[1] == S.MAX_PAGES
+    with pytest.raises(ValueError, match="max_seq"):
+        Engine(ecfg, max_seq=widest + 1, global_pages=8)
