@@ -46,7 +46,6 @@ struct Lane {
 
 template <int BYTES>
 struct Raw;
-template <> struct Raw<1> { using T = uint8_t; };
 template <> struct Raw<2> { using T = uint16_t; };
 template <> struct Raw<4> { using T = uint32_t; };
 
@@ -81,9 +80,7 @@ struct Head {
 };
 template <int P>
 __device__ __forceinline__ void load_words(const void* src, uint32_t* w) {
-  if constexpr (P == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(src);
-  } else if constexpr (P == 2) {
+  if constexpr (P == 2) {
     const uint2 v = *reinterpret_cast<const uint2*>(src);
     w[0] = v.x;
     w[1] = v.y;
@@ -155,20 +152,16 @@ __device__ __forceinline__ Head<D> store_row(uint8_t* part, int off, int lane, f
       for (int j = 0; j < P; ++j) out.w[hh * P + j] = to_bf2(x[hh * P + j]);
       store_words<P>(part + off * 2 * D + kv_swizzle_byte(2 * e0, off, 2 * D), &out.w[hh * P]);
     } else if constexpr (FMT == kKvFp8) {
-      uint32_t word[P > 1 ? P / 2 : 1] = {};
+      uint32_t word[P / 2] = {};
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         const uint32_t e = f32x2_to_e4m3x2(x[hh * P + j].x * inv, x[hh * P + j].y * inv);
         out.w[hh * P + j] = e4m3x2_to_f16x2(static_cast<uint16_t>(e));
         word[j / 2] |= e << (16 * (j & 1));
       }
-      uint8_t* dst = part + off * D + kv_swizzle_byte(e0, off, D);
-      if constexpr (P == 1) *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(word[0]);
-      else if constexpr (P == 2) *reinterpret_cast<uint32_t*>(dst) = word[0];
-      else *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
+      *reinterpret_cast<uint2*>(part + off * D + kv_swizzle_byte(e0, off, D)) = make_uint2(word[0], word[1]);
     } else {
       constexpr int LPB = 16 / H2;       // lanes per 16-value block
-      using T = typename Raw<(H2 / 2 > 0 ? H2 / 2 : 1)>::T;
       float2 y[P];
       float amax = 0.f;
 #pragma unroll
@@ -185,7 +178,7 @@ __device__ __forceinline__ Head<D> store_row(uint8_t* part, int off, int lane, f
 #pragma unroll
       for (int j = 0; j < P; ++j)
         word |= (e2m1_code(y[j].x * inv_sf) | (e2m1_code(y[j].y * inv_sf) << 4)) << (8 * j);
-      *reinterpret_cast<T*>(part + off * (D / 2) + kv_swizzle_byte(e0 / 2, off, D / 2)) = static_cast<T>(word);
+      *reinterpret_cast<uint32_t*>(part + off * (D / 2) + kv_swizzle_byte(e0 / 2, off, D / 2)) = word;
       widen_e2m1<H2>(word, sf, &out.w[hh * P]);
     }
   }
@@ -202,18 +195,13 @@ __device__ __forceinline__ Head<D> load_row(const uint8_t* part, int off, int la
     if constexpr (FMT == kKvBf16) {
       load_words<P>(part + off * 2 * D + kv_swizzle_byte(2 * e0, off, 2 * D), &out.w[hh * P]);
     } else if constexpr (FMT == kKvFp8) {
-      const uint8_t* src = part + off * D + kv_swizzle_byte(e0, off, D);
-      uint2 word = make_uint2(0, 0);
-      if constexpr (P == 1) word.x = *reinterpret_cast<const uint16_t*>(src);
-      else if constexpr (P == 2) word.x = *reinterpret_cast<const uint32_t*>(src);
-      else word = *reinterpret_cast<const uint2*>(src);
+      const uint2 word = *reinterpret_cast<const uint2*>(part + off * D + kv_swizzle_byte(e0, off, D));
 #pragma unroll
       for (int j = 0; j < P; ++j)
         out.w[hh * P + j] = e4m3x2_to_f16x2(static_cast<uint16_t>((j < 2 ? word.x : word.y) >> (16 * (j & 1))));
     } else {
-      using T = typename Raw<(H2 / 2 > 0 ? H2 / 2 : 1)>::T;
       const float sf = e4m3_to_float(part[kPage * (D / 2) + off * (D / 16) + e0 / 16]);
-      const uint32_t word = *reinterpret_cast<const T*>(part + off * (D / 2) + kv_swizzle_byte(e0 / 2, off, D / 2));
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(part + off * (D / 2) + kv_swizzle_byte(e0 / 2, off, D / 2));
       widen_e2m1<H2>(word, sf, &out.w[hh * P]);
     }
   }
@@ -227,18 +215,13 @@ struct Angles {
   __device__ __forceinline__ void load(const float* cs, int lane) {
     constexpr int H2 = Lane<D>::H2;
     const float* cl = cs + lane * H2;
-    if constexpr (H2 == 2) {
-      c[0] = *reinterpret_cast<const float2*>(cl);
-      s[0] = *reinterpret_cast<const float2*>(cl + D / 2);
-    } else {
 #pragma unroll
-      for (int j = 0; j < H2; j += 4) {
-        const float4 u = *reinterpret_cast<const float4*>(cl + j), v = *reinterpret_cast<const float4*>(cl + D / 2 + j);
-        c[j / 2] = make_float2(u.x, u.y);
-        c[j / 2 + 1] = make_float2(u.z, u.w);
-        s[j / 2] = make_float2(v.x, v.y);
-        s[j / 2 + 1] = make_float2(v.z, v.w);
-      }
+    for (int j = 0; j < H2; j += 4) {
+      const float4 u = *reinterpret_cast<const float4*>(cl + j), v = *reinterpret_cast<const float4*>(cl + D / 2 + j);
+      c[j / 2] = make_float2(u.x, u.y);
+      c[j / 2 + 1] = make_float2(u.z, u.w);
+      s[j / 2] = make_float2(v.x, v.y);
+      s[j / 2 + 1] = make_float2(v.z, v.w);
     }
 #pragma unroll
     for (int j = 0; j < H2 / 2; ++j) ns[j] = make_float2(-s[j].x, -s[j].y);
