@@ -546,7 +546,10 @@ class GQARunner:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, pool=self.graph_pool):
             body()
-        return g.replay
+
+        def replay(keep=body):           # the graph reads tensors that the body closes over: they live as long as it
+            g.replay()
+        return replay
 
     # ------------------------------------------------------------------------------------------ speculative
     # EAGLE-style greedy speculation with a one-layer draft head (`speculative/` in the reference; semantics of a

@@ -110,3 +110,32 @@ def test_two_ranks():
                 assert tok == int(ref.argmax())
                 checked += 1
     assert checked >= 6
+
+
+def test_a_captured_step_keeps_the_tensors_that_it_reads(monkeypatch):
+    """A graph holds addresses: what a step body made before its capture must not be freed while the graph can replay."""
+    import contextlib
+    import gc
+    import weakref
+    fake = type("Fake", (), {"wait_stream": lambda *a: None, "replay": lambda *a: None})
+    monkeypatch.setattr(torch.cuda, "Stream", lambda *a, **k: fake())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a, **k: fake())
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "graph", lambda g, pool=None: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", fake)
+    monkeypatch.setattr(torch.cuda, "graph_pool_handle", lambda: 0)
+    run = _engine().runner
+    rows = torch.arange(4)
+    ran = []
+
+    def body(rows=rows):
+        ran.append(rows.sum().item())
+    left = weakref.ref(rows)
+    step = run._capture(body)
+    del rows, body
+    gc.collect()
+    assert left() is not None and ran == [6, 6]
+    step()
+    del step
+    gc.collect()
+    assert left() is None
