@@ -146,21 +146,6 @@ __device__ __forceinline__ float2 in_units(float2 x, float unit, float inv) {
   const float2 c = fma2(fma2(q, make_float2(-unit, -unit), x), make_float2(inv, inv), q);
   return make_float2(fabsf(q.x) < INFINITY ? c.x : q.x, fabsf(q.y) < INFINITY ? c.y : q.y);
 }
-// E2M1 codes of 8 values of one block, lowest nibble first: a magnitude's code is the number of midpoints strictly below
-// it, compared as midpoint x block scale, which is exact (`e2m1_code` of the quotient, without 8 divisions).
-__device__ __forceinline__ uint32_t e2m1_word(const float2 (&y)[4], float sf) {
-  const float mid[7] = {0.25f * sf, 0.75f * sf, 1.25f * sf, 1.75f * sf, 2.5f * sf, 3.5f * sf, 5.f * sf};
-  uint32_t word = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float v = (j & 1) ? y[j / 2].y : y[j / 2].x, a = fabsf(v);
-    uint32_t m = 0;
-#pragma unroll
-    for (int k = 0; k < 7; ++k) m += a > mid[k];
-    word |= (m | ((v < 0.f && m > 0) ? 8u : 0u)) << (4 * j);
-  }
-  return word;
-}
 
 // One row of a pool part (K or V of a page and head): stores x (one rounding, from fp32; `unit` is the pool's scale, `inv` its
 // reciprocal) and returns what the row holds.
@@ -198,9 +183,14 @@ __device__ __forceinline__ Head<D> store_row(uint8_t* part, int off, int lane, f
 #pragma unroll
       for (int o = 1; o < LPB; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(Lane<D>::mask(), amax, o));
       const uint8_t s8 = nvfp4_block_scale(amax);
-      const float sf = e4m3_to_float(s8);
+      // E2M1 codes count the midpoints strictly below a magnitude (ties go down), so a reciprocal rounded down keeps a value
+      // that is a midpoint times the block's scale on the right side
+      const float sf = e4m3_to_float(s8), inv_sf = __frcp_rd(sf);
       if ((lane % LPB) == 0) part[kPage * (D / 2) + off * (D / 16) + e0 / 16] = s8;
-      const uint32_t word = e2m1_word(y, sf);
+      uint32_t word = 0;
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        word |= (e2m1_code(y[j].x * inv_sf) | (e2m1_code(y[j].y * inv_sf) << 4)) << (8 * j);
       *reinterpret_cast<uint32_t*>(part + off * (D / 2) + kv_swizzle_byte(e0 / 2, off, D / 2)) = word;
       widen_e2m1<H2>(word, sf, &out.w[hh * P]);
     }
