@@ -16,10 +16,11 @@
 // columns permuted alike, and V's values as the row order of O^T they arrive in, undone when O is stored.  8-bit and
 // 4-bit values are widened to f16 (exactly, block scales included) between shared memory and the fragments.
 //
-// Bound by the listed pages' bytes over bf16 and E4M3 caches (16 x 16 lists of 32 pages of D = 512, bf16: 144 us, 6.7
-// TB/s; 64 x 8 lists of D = 128, E4M3: 49.5 us, 5.4 TB/s), by the conversions over FP4 caches (32 x 16 lists of 64 pages
-// of D = 512: 266 us, 4.3 TB/s), by launch and load latency for one user (8 lists of 32 pages of D = 128: 8.0 us), by the
-// path from L2 for a prefill's groups (512 x 8 lists of 32 pages, 4.3 GB, of a 35k-token request: 361 us).
+// Bound by the listed pages' bytes over bf16 and E4M3 caches (16 x 16 lists of 32 pages of D = 512, bf16: 143 us, 6.7
+// TB/s; 64 x 8 lists of D = 128, E4M3: 49.5 us, 5.4 TB/s).  Over FP4 caches by latency that 8 warps an SM do not hide, no
+// pipe being full (32 x 16 lists of 64 pages of D = 512: 266 us, 4.3 TB/s; issue slots and ALU under 50 %), for one user by
+// launch and load latency (8 lists of 32 pages of D = 128: 7.9 us), for a prefill's groups by the path from L2 and the
+// products (512 x 8 lists of 32 pages, 4.3 GB, of a 35k-token request: 375 us, 440 once the power cap takes the clock down).
 #include "common.cuh"
 #include "kernels.h"
 
@@ -54,9 +55,9 @@ struct Cfg {
   static constexpr int SC = FMT == kKvNvfp4 ? D / 16 : 0;                 // block scale bytes of a row
   // Bytes of a tile (at least 16 tokens, at most a page) and CTAs of an SM, which the registers bound (Q and O take
   // D / 8 * NR + D / 4 * NR of a thread's).  Larger tiles spread a step's fixed cost, more CTAs hide latencies.
-  // Measured, 8 KB with 3 CTAs against 4 KB with 4 (D = 128, one column group): bf16 32 x 8 x 32 pages 43.5 / 45.3 us,
-  // E4M3 64 x 8 x 32 pages 60.0 / 50.0 us, FP4 the same lists 48.4 / 42.4 us; two column groups, bf16 512 x 8 x 32
-  // pages 319 / 483 us.  D = 512, FP4, 32 x 16 x 64 pages: 8 KB 280 us, 4 KB 319 us.
+  // Measured, 8 KB with 3 CTAs against 4 KB with 4 (D = 128, one column group): bf16 32 x 8 x 32 pages 43.4 / 45.4 us,
+  // E4M3 64 x 8 x 32 pages 59.0 / 49.5 us, FP4 the same lists 46.6 / 40.9 us; two column groups, bf16 512 x 8 x 32
+  // pages 375 / 478 us.  D = 512, FP4, 32 x 16 x 64 pages: 8 KB 266 us, 4 KB 306 us.
   static constexpr bool SMALL = D == 128 && NR == 1 && !BF;
   static constexpr int TB = SMALL ? 4096 : 8192;
   static constexpr int ST = TB / RB < 16 ? 16 : TB / RB < 64 ? TB / RB : 64;
@@ -70,8 +71,8 @@ struct Cfg {
   static constexpr int MT = D / 16;                        // 16-value tiles of O^T
   static constexpr int DP = D + 4;                         // floats between rows of a partial output
   // Over FP4 caches Q's operand registers stay in shared memory where O takes 128 of a thread's: 64 more would leave
-  // too few to overlap the conversions (D = 512, 32 x 16 x 64 pages: 271 against 278 us; over 8-bit and 16-bit caches,
-  // bound by their bytes, registers are better: D = 512, bf16, 16 x 16 x 32 pages 151 against 144 us).
+  // too few to overlap the conversions (D = 512, 32 x 16 x 64 pages: 266 against 280 us; over 8-bit and 16-bit caches,
+  // bound by their bytes, registers are better: when it was chosen, D = 512, bf16, 16 x 16 x 32 pages 151 against 144 us).
   static constexpr bool QSM = D * NR >= 512 && FMT == kKvNvfp4;
   static constexpr int QB = QSM ? KK * NR * 256 : 0;       // bytes of it
   static constexpr int RES = SLOT > 12000 ? 1 : D * NR >= 512 ? 2 : SMALL ? 4 : 3;

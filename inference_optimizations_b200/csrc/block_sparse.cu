@@ -388,8 +388,9 @@ __device__ void finish_bound(const Bound<D, FMT>& bd, float unit, int8_t* codes,
 // one page): its warps share the run's rows, and when the run ends at the page's last row the CTA also reads the rows
 // written by earlier calls and writes the page's bound, so the bound costs no launch and no second pass over the new
 // keys.
-// Bound by bytes: 8192 rows, 32 q and 16 kv heads of 512, bf16: 202 us for 1.09 GB (5.4 TB/s); a step of 64 rows is
-// bound by its chain of loads: 5.5 us, 7.5 MB.  Mixing a slab's K and q / v CTAs in launch order instead of all K first:
+// Bound by bytes: 8192 rows, 32 q and 16 kv heads of 512, bf16: 205 us for 1.09 GB (5.3 TB/s), E4M3 196 us for 0.96 GB;
+// over FP4 caches by the encoding (309 us for 0.90 GB).  A step of 64 rows is bound by its chain of loads: 5.8 us, 7.5 MB,
+// E4M3; FP4 9.3.  Mixing a slab's K and q / v CTAs in launch order instead of all K first:
 // 205 against 214 us; 8 warps a CTA instead of 4: 330.
 __device__ __forceinline__ int row_slot(const BlockAppendArgs& a, int t) {
   const int s = a.slot[t], p = a.pos[t];
@@ -532,7 +533,7 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 // bits, which would put every key in one bin), ending as soon as a digit's bin is taken whole.
 // Bound by bytes for a batch (32 groups x 16 heads x up to 512 pages of D = 512: 38 us for 175 MB, 4.6 TB/s, the
 // selection's few microseconds behind the last score included), by latency for one user (8 heads x 3200 pages of
-// D = 128: 10.4 us, 6.6 MB), by issue for a prefill's many lists (512 x 8 x 544 pages of D = 128: 79 us).
+// D = 128: 10.5 us, 6.6 MB), by issue for a prefill's many lists (512 x 8 x 544 pages of D = 128: 79 us).
 template <int D, bool R8, int NT, int PP, int RES>
 __global__ void __launch_bounds__(NT, RES) block_select_kernel(const BlockSelectArgs a, const int csize) {
   constexpr int RS = 2 * D + 64;        // bytes between query rows
@@ -823,9 +824,9 @@ cudaError_t select_launch_r(const BlockSelectArgs& a, cudaStream_t s) {
   // scores.  Enough to fill the SMs twice over: the same with larger CTAs; up to twice: with twice as large ones, whose
   // selection is shorter.  Few: the candidates of a list are split over a cluster until the SMs have two CTAs each, as
   // long as a CTA keeps 64 pages, with 16 loads in flight per thread.  (The page table's width bounds the candidates.)
-  // Measured, many / some / few: 512 groups x 8 heads x 544 pages of D = 128: 84 / 98 / 141 us; 32 x 16 x 512 pages of
-  // D = 512: 50 / 38 / 45 us; 1 x 8 x 3200 pages of D = 128: 56 / 32 / 10 us; some with 256 / 512 threads: 32 x 16 lists
-  // 38 / 42 us, 16 x 16 lists 28 / 23 us.
+  // Measured, many / some / few: 512 groups x 8 heads x 544 pages of D = 128: 79 / 93 / 134 us; 32 x 16 x 512 pages of
+  // D = 512: 50 / 38 / 45 us; 1 x 8 x 3200 pages of D = 128: 56 / 32 / 11 us; some with 256 / 512 threads: 32 x 16 lists
+  // 38 / 43 us, 16 x 16 lists 29 / 23 us.
   const int units = a.B * a.Hk;
   const int var = units >= 148 * 8 ? 2 : units > 148 ? 1 : 0;
   int cs = 1;
@@ -860,10 +861,14 @@ cudaError_t block_append(const BlockAppendArgs& a_, cudaStream_t s) {
   BlockAppendArgs a = a_;
   if (a.T == 0) return cudaSuccess;
   if (a.T > 65535 * 16) return cudaErrorInvalidValue;      // the grid's second dimension
-  // A decode step (few rows, each its own page) wants a CTA per row; a prefill wants fewer, longer CTAs.
+  // A decode step (each row its own page) wants a CTA per row, a prefill fewer, longer CTAs.  The number of rows stands for
+  // both.  Measured, a row / 16 rows a CTA: steps of 200 rows of D = 512, E4M3 14.8 / 22.7 us; verify of 32 x 4 rows
+  // 8.5 / 9.4, of 64 x 4 16.6 / 12.7, of 65 x 4 of D = 128, bf16 6.3 / 6.9, of 200 x 4 14.3 / 9.5; one request of 100 rows of
+  // D = 512, bf16 9.8 / 10.2, of 300 22.9 / 17.7, of 512 32.6 / 21.1.
   a.slab = a.T <= 256 ? 1 : 16;
   // Heads of a q / v CTA: one per vector of its warps for a step; in a prefill a warp walks through 4 (D = 512) or through
-  // 2 vectors' worth, which shares the angles and keeps enough CTAs (7 x 219 rows of D = 256: 26.1 us, twice as many 28.0).
+  // 2 vectors' worth, which shares the angles and keeps enough CTAs (7 x 219 rows of D = 256, E4M3: 26.1 us when it was chosen,
+  // twice as many heads 28.0).
   a.heads = a.slab == 1 ? 4 * (512 / a.D) : a.D == 512 ? 4 : 2 * (512 / a.D);
   IOB_BY_D_FMT(append_launch, a, s)
 }

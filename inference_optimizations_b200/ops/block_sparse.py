@@ -66,8 +66,9 @@ def block_append(qkv: torch.Tensor, q_norm: Optional[torch.Tensor], k_norm: Opti
     [T, Hq, D] (returned), k and v -> pool[slot] in the pool's format; everything in fp32 with one rounding at the end
     (`gqa_prep` rounds to bf16 after the norm).  Every page whose last row (slot % 64 == 63) is written gets its key
     bounds.  A row with slot -1, or with a position outside the table, is not written (its q is zero in the latter
-    case).  E4M3 values saturate.  Rows of one page are adjacent and ascending in a call, and its earlier rows were written by earlier calls
-    on the stream: the order in which a request's tokens arrive."""
+    case).  E4M3 values saturate.  Rows of one page are adjacent and ascending in a call, without a row that is not
+    written between them, and the page's earlier rows were written by earlier calls on the stream: the order in which a
+    request's tokens arrive.  V's bytes are those of `gqa_prep`; K's may differ in the last bit (one rounding, not two)."""
     if qkv.is_cuda:
         return ext().block_append(qkv, q_norm, k_norm, cos_sin, pos, slot, q_out, pool, codes, scale, fmt, k_scale,
                                   v_scale, hq, hk, d, eps, plus_one)
@@ -208,7 +209,11 @@ def block_decode(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
     log).  blocks int32 [B, Hk, budget] from `block_select` or any list of logical pages in any order, each at most
     once; entries < 0, past kv_len or without a page of the pool are skipped.  What the cache holds past kv_len is
     never used, whatever it is.  k_scale / v_scale are ignored on bf16 pools.  status int32 [1]: a copy that did not
-    arrive within the wait limit records a code there (and the group's output is NaN)."""
+    arrive within the wait limit records a code there (and the group's output is NaN).
+
+    Accuracy: scores and sums are fp32; a weight enters the product with V in 11 bits over 8-bit and 4-bit caches (to
+    2^-26 of the row's largest, 2^-37 of it below), in 16 bits over bf16 caches; the output is rounded to bf16.  A value of
+    V that is not finite reaches the rows that see it and no other."""
     if q.is_cuda:
         return ext().block_decode(q, pool, page_table, req_idx, kv_len, blocks, out, lse, status, n_q, hk, fmt,
                                   sm_scale, k_scale, v_scale)
